@@ -54,7 +54,15 @@ enum {
     TGRU_E_ALIGN = -4,     /* a buffer is not 16-byte aligned */
     TGRU_E_LAUNCH = -5,    /* a kernel launch failed; hipGetLastError() has the cause */
     TGRU_E_NOGPU = -6,     /* the current device is not a gfx950 GPU */
-    TGRU_E_TOOBIG = -7     /* tgru_forward_static: the call needs more than TGRU_STATIC_WORKSPACE_BYTES */
+    TGRU_E_TOOBIG = -7,    /* tgru_forward_static: the call needs more than TGRU_STATIC_WORKSPACE_BYTES */
+    TGRU_E_DTYPE = -8      /* a dtype that is none of TGRU_DTYPE_* */
+};
+
+/* Element types of the sequence tensors of the state-space operators below (everything else is fp32). */
+enum {
+    TGRU_DTYPE_F32 = 0,
+    TGRU_DTYPE_BF16 = 1,
+    TGRU_DTYPE_F16 = 2
 };
 
 /* Library version (major*10000 + minor*100 + patch).  No reference counterpart. */
@@ -412,6 +420,118 @@ int tgru_loss_backward(int kind, const float *const *in, float *const *din, cons
  */
 int tgru_uniform(float *out, long n, unsigned long long seed, unsigned long long stream,
                  unsigned long long first, tgru_stream_t s);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * State-space sequence operators: the short causal convolution and the selective scan of a state-space layer, the
+ * other recurrent layer of this library (the GRU above is one; the reference has no counterpart of these).
+ *
+ * Sequence tensors (x, u, delta, z, y and their gradients (B, T, D); b, c and theirs (B, T, G, N)) have the element
+ * type `dtype` and any non-negative element strides over sequences, steps and groups, consecutive elements in the
+ * last dimension; inputs may be broadcast (stride 0), outputs may not overlap themselves.  Parameters, their
+ * gradients and scan states are fp32 and dense.  All arithmetic is fp32; outputs are rounded once.
+ * lengths: device int32[B] or NULL; sequence b has clamp(lengths[b], 0, T) steps, in any order of lengths, zero
+ * included.  Rows behind a sequence's end are never looked at (they may hold NaN); outputs and gradients there are 0.
+ * No output may overlap an input or another output, except where said.
+ * Every result is the same from call to call (no atomics).  Pointers need the alignment of their element type only.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/*
+ * y_t[d] = act(bias[d] + sum_k weight[d][k] x_{t-K+1+k}[d]), act(v) = v / (1 + exp(-v)) if `silu`, else v.
+ * 1 <= K <= TGRU_CONV_MAX_TAPS.  x before the first step is initial_state (B, K-1, D; rows in order of time, dense,
+ * `dtype`), 0 where that is NULL.  final_state (same shape, or NULL): the K-1 inputs before position length, what
+ * the next call's initial_state, or tgru_conv_step, goes on from.
+ * Backward: from dy (or NULL: zeros) and dfinal (gradient of final_state, or NULL) the gradients dx, dinitial,
+ * dweight (D, K), dbias (D), each NULL where not wanted; x, weight, bias, initial_state, lengths as in the forward
+ * call.  `workspace`: tgru_conv_backward_workspace_bytes() bytes, needed where dweight or dbias is wanted.
+ */
+#define TGRU_CONV_MAX_TAPS 8
+typedef struct tgru_conv_args {
+    const void *x;
+    const float *weight, *bias;
+    const void *initial_state;
+    const int32_t *lengths;
+    void *y, *final_state;
+    const void *dy, *dfinal;
+    void *dx, *dinitial;
+    float *dweight, *dbias;
+    float *workspace;
+    int64_t x_stride[2], y_stride[2], dy_stride[2], dx_stride[2];   /* elements from sequence to sequence, step to step */
+    int32_t B, T, D, K, dtype, silu;
+} tgru_conv_args;
+int tgru_conv_forward(const tgru_conv_args *a, tgru_stream_t stream);
+int tgru_conv_backward(const tgru_conv_args *a, tgru_stream_t stream);
+size_t tgru_conv_backward_workspace_bytes(int B, int T, int D, int K);
+
+/*
+ * One more step of the convolution for each of B sequences whose states lie in a pool: y (B, D) from x (B, D) and
+ * state[slots[i]] (pool of P states (K-1, D) of `dtype`), whose rows move up by one and take x as the last; the new
+ * state goes to state_out[slots[i]] (state_out == state: in place; any other overlap is an error of the caller).
+ * slots: device int32[B], or NULL: row i has state i (then P >= B).  A row whose slot is outside [0, P) is padding:
+ * y is 0 there and no state is touched.  Rows with the same slot are taken one after the other, in order of rows.
+ */
+typedef struct tgru_conv_step_args {
+    const void *x;
+    const void *state;
+    void *state_out;
+    const float *weight, *bias;
+    const int32_t *slots;
+    void *y;
+    int64_t x_stride, y_stride;                  /* elements from row to row */
+    int32_t B, P, D, K, dtype, silu;
+} tgru_conv_step_args;
+int tgru_conv_step(const tgru_conv_step_args *a, tgru_stream_t stream);
+
+/*
+ * The selective scan.  For every sequence and channel d, with the N states of a channel as vectors,
+ *     dt_t = softplus(delta_t + delta_bias)        (delta_t + delta_bias without `softplus`)
+ *     h_t  = exp(dt_t A[d]) h_{t-1} + dt_t u_t b_t[group of d]
+ *     y_t  = (c_t[group of d] . h_t + skip[d] u_t) z_t / (1 + exp(-z_t))
+ * a (D, N); 1 <= N <= TGRU_SCAN_MAX_STATES; G divides D, group of d = d / (D / G).  skip, delta_bias and z may be NULL
+ * (no such term / factor).  initial_state / final_state (B, D, N) fp32, NULL: zeros / not wanted.
+ * reserve: tgru_scan_reserve_bytes() bytes that the backward call reads, or NULL (inference).
+ * Backward: from dy (or NULL: zeros) and dfinal (or NULL) the gradients du, ddelta, dz, db, dc, da, dskip, ddelta_bias,
+ * dinitial, each NULL where not wanted; the inputs as in the forward call.  db and dc are dense (B, T, G, N).
+ * `workspace`: tgru_scan_workspace_bytes(..., backward) bytes.
+ */
+#define TGRU_SCAN_MAX_STATES 64
+typedef struct tgru_scan_args {
+    const void *u, *delta, *z, *b, *c;
+    const float *a, *skip, *delta_bias;
+    const float *initial_state;
+    const int32_t *lengths;
+    void *y;
+    float *final_state;
+    float *reserve, *workspace;
+    const void *dy;
+    const float *dfinal;
+    void *du, *ddelta, *dz, *db, *dc;
+    float *da, *dskip, *ddelta_bias, *dinitial;
+    int64_t u_stride[2], delta_stride[2], z_stride[2], y_stride[2], dy_stride[2], du_stride[2], ddelta_stride[2],
+            dz_stride[2];                        /* elements from sequence to sequence, step to step */
+    int64_t b_stride[3], c_stride[3];            /* ... and from group to group */
+    int32_t B, T, D, N, G, dtype, softplus;
+} tgru_scan_args;
+int tgru_scan_forward(const tgru_scan_args *a, tgru_stream_t stream);
+int tgru_scan_backward(const tgru_scan_args *a, tgru_stream_t stream);
+size_t tgru_scan_reserve_bytes(int B, int T, int D, int N, int G);
+size_t tgru_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward);
+
+/*
+ * One more step of the scan for each of B sequences whose states (D, N) fp32 lie in a pool of P; slots, padding rows,
+ * repeated slots, state and state_out as in tgru_conv_step.  u, delta, z, y (B, D), b, c (B, G, N).
+ */
+typedef struct tgru_scan_step_args {
+    const void *u, *delta, *z, *b, *c;
+    const float *a, *skip, *delta_bias;
+    const float *state;
+    float *state_out;
+    const int32_t *slots;
+    void *y;
+    int64_t u_stride, delta_stride, z_stride, y_stride;   /* elements from row to row */
+    int64_t b_stride[2], c_stride[2];                     /* ... and from group to group */
+    int32_t B, P, D, N, G, dtype, softplus;
+} tgru_scan_step_args;
+int tgru_scan_step(const tgru_scan_step_args *a, tgru_stream_t stream);
 
 #ifdef __cplusplus
 }

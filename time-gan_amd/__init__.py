@@ -3,6 +3,8 @@ from ._lib import (TgruError, lib, LAYOUT_TBF, LAYOUT_BTF, LAYOUT_PACKED,  # noq
                    reload_switches, launch_count, persist_timeouts, check_persist_timeouts)
 from .functional import GRURunner, gru_forward_backward_raw, gru_apply, input_projection  # noqa: F401
 from .gru import GRU  # noqa: F401
+from .ssm import (SSM, SSMState, selective_scan, selective_scan_step, short_conv,  # noqa: F401
+                  short_conv_step)
 from .modules import (Embedding, Recovery, Supervisor, Generator, Discriminator,  # noqa: F401
                       build_networks, make_cfg)
 from . import data, losses, parallel, scorer  # noqa: F401

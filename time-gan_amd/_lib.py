@@ -54,6 +54,43 @@ class AdamJob(ctypes.Structure):
                [("n", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+_SEQ = ctypes.c_int64 * 2
+_MAP = ctypes.c_int64 * 3
+
+
+class ConvArgs(ctypes.Structure):
+    """tgru_conv_args of include/tgru.h."""
+    _fields_ = [(n, _vp) for n in ("x", "weight", "bias", "initial_state", "lengths", "y", "final_state", "dy", "dfinal",
+                                   "dx", "dinitial", "dweight", "dbias", "workspace")] + \
+               [(n, _SEQ) for n in ("x_stride", "y_stride", "dy_stride", "dx_stride")] + \
+               [(n, ctypes.c_int32) for n in ("B", "T", "D", "K", "dtype", "silu")]
+
+
+class ConvStepArgs(ctypes.Structure):
+    """tgru_conv_step_args of include/tgru.h."""
+    _fields_ = [(n, _vp) for n in ("x", "state", "state_out", "weight", "bias", "slots", "y")] + \
+               [("x_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("B", "P", "D", "K", "dtype", "silu")]
+
+
+class ScanArgs(ctypes.Structure):
+    """tgru_scan_args of include/tgru.h."""
+    _fields_ = [(n, _vp) for n in ("u", "delta", "z", "b", "c", "a", "skip", "delta_bias", "initial_state", "lengths", "y",
+                                   "final_state", "reserve", "workspace", "dy", "dfinal", "du", "ddelta", "dz", "db", "dc",
+                                   "da", "dskip", "ddelta_bias", "dinitial")] + \
+               [(n + "_stride", _SEQ) for n in ("u", "delta", "z", "y", "dy", "du", "ddelta", "dz")] + \
+               [("b_stride", _MAP), ("c_stride", _MAP)] + \
+               [(n, ctypes.c_int32) for n in ("B", "T", "D", "N", "G", "dtype", "softplus")]
+
+
+class ScanStepArgs(ctypes.Structure):
+    """tgru_scan_step_args of include/tgru.h."""
+    _fields_ = [(n, _vp) for n in ("u", "delta", "z", "b", "c", "a", "skip", "delta_bias", "state", "state_out", "slots", "y")] + \
+               [(n + "_stride", ctypes.c_int64) for n in ("u", "delta", "z", "y")] + \
+               [("b_stride", _SEQ), ("c_stride", _SEQ)] + \
+               [(n, ctypes.c_int32) for n in ("B", "P", "D", "N", "G", "dtype", "softplus")]
+
+
 MAX_ADAM_JOBS = 64        # TGRU_MAX_ADAM_JOBS
 MAX_ADAM_ELEMS = 65536    # TGRU_MAX_ADAM_ELEMS
 DEFER_REDUCE = 2          # TGRU_DEFER_REDUCE
@@ -99,6 +136,15 @@ SIGNATURES = {
     "tgru_reduce_jobs": (_i, [ctypes.POINTER(ReduceJob), _i, _vp]),
     "tgru_adam_jobs": (_i, [ctypes.POINTER(AdamJob), _i] + [ctypes.c_float] * 4 + [_vp, _vp]),
     "tgru_uniform": (_i, [_vp, ctypes.c_long, ctypes.c_ulonglong, ctypes.c_ulonglong, ctypes.c_ulonglong, _vp]),
+    "tgru_conv_forward": (_i, [ctypes.POINTER(ConvArgs), _vp]),
+    "tgru_conv_backward": (_i, [ctypes.POINTER(ConvArgs), _vp]),
+    "tgru_conv_backward_workspace_bytes": (ctypes.c_size_t, [_i] * 4),
+    "tgru_conv_step": (_i, [ctypes.POINTER(ConvStepArgs), _vp]),
+    "tgru_scan_forward": (_i, [ctypes.POINTER(ScanArgs), _vp]),
+    "tgru_scan_backward": (_i, [ctypes.POINTER(ScanArgs), _vp]),
+    "tgru_scan_reserve_bytes": (ctypes.c_size_t, [_i] * 5),
+    "tgru_scan_workspace_bytes": (ctypes.c_size_t, [_i] * 6),
+    "tgru_scan_step": (_i, [ctypes.POINTER(ScanStepArgs), _vp]),
     "tgru_loss_layout": (_i, [_i] * 3 + [ctypes.POINTER(ctypes.c_int64)]),
     "tgru_loss_partial": (_i, [_i, _i, _vp] + [_i] * 4 + [_vp, _vp]),
     "tgru_loss_final": (_i, [_i] * 5 + [ctypes.c_float, _vp, _vp]),

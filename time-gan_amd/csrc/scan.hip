@@ -1,0 +1,831 @@
+// Selective scan: h_t = exp(dt_t A) h_{t-1} + dt_t u_t b_t, y_t = (c_t . h_t + skip u_t) silu(z_t) for every channel (N
+// states each), its backward pass, and its form for one more token on a pool of states (tgru_scan_* of
+// include/tgru.h).
+//
+// What bounds it.  A step costs, per channel AND STATE, one exponential and four multiply-adds forward, and about
+// eighteen operations and the exponential backward, against a few bytes per channel: with 16 states the vector ALU and
+// not HBM is the limit.  The matrix instructions do not apply: every (channel, state) pair has a decay of its own at
+// every step, so no product of two matrices is shared by two steps.  Hence:
+//   * the exponentials are computed once per pass and kept in registers where the backward pass needs them again;
+//   * everything that is per channel only (softplus, dt u, the gate) is computed once per (step, channel), by lanes that
+//     split a block of 16 steps among themselves, and handed to the recurrence through LDS;
+//   * sums over the states of a channel and over the channels of a group are joined inside the wave with DPP adds and
+//     permlane swaps.
+//
+// Layout.  A wave owns CH = 64 / S channels: S lanes per channel, four states each (S = 1, 2, 4, 8, 16 covers 64 states;
+// states beyond N are zeros throughout).  Lane = channel * S + part.  A block of Q = 16 steps is staged in LDS (dt, dt u,
+// b, c in fp32), the next block's rows are requested before the recurrence runs over this one.  Nothing is shared between
+// waves in the forward pass: there is no barrier.
+//
+// Time is split into chunks when there are too few channels to fill the chip (chunk_plan): a first pass leaves each
+// chunk's end state from a zero start and its sum of dt -- the chunk multiplies an incoming state by exp(A sum dt) --, a
+// second kernel joins the chunks in order, and the main pass starts every chunk from its joined state.  The backward
+// pass does the same from the other end.
+//
+// For the backward pass the forward pass saves the state in front of every block of 16 steps (4 bytes per step, channel
+// and 16 states); the states inside a block are computed again from it, 16 steps in registers at a time.
+#include "ssm_common.h"
+#include <type_traits>
+
+namespace tgru {
+namespace ssm {
+
+constexpr int Q = 16;                // steps per block
+constexpr int kWaves = 4;            // per workgroup
+
+struct Plan {                        // how a call is cut up; made on the host
+    int S, CH;                       // lanes per channel, channels per wave
+    int Dg, tpg, tiles;              // channels per group, waves per group, waves per sequence and chunk
+    int wpg;                         // backward: workgroups per group
+    int nblk;                        // blocks of Q steps
+    int nchunks, chunk;              // chunks of time, steps of one (a multiple of Q)
+};
+
+// What goes between kernels, per wave-lane: float4 carry[b][chunk][tile][64], float sdt[b][chunk][tile][64],
+// float4 ckpt[b][block][tile][64].
+__device__ __forceinline__ long lane_slot(const Plan &pl, int b, int outer, int nouter, int tile) {
+    return (((long)b * nouter + outer) * pl.tiles + tile) * 64 + (threadIdx.x & 63);
+}
+
+// LDS written by some lanes of a wave and read by others: the LDS unit takes a wave's accesses in order, so all that
+// has to be held back is the compiler.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// Sum over the S lanes of a channel, in every one of them.
+template <int S>
+__device__ __forceinline__ float sum_parts(float v) {
+    if constexpr (S >= 2) v = dpp_add<0xB1>(v);      // quad_perm [1,0,3,2]
+    if constexpr (S >= 4) v = dpp_add<0x4E>(v);      // quad_perm [2,3,0,1]
+    if constexpr (S >= 8) v = dpp_add<0x141>(v);     // row_half_mirror
+    if constexpr (S >= 16) v = dpp_add<0x140>(v);    // row_mirror
+    return v;
+}
+// Sums over the CH channels of a wave of four values v[0..3] per lane.  The lanes' two top bits are taken by swapping
+// halves and quarters (which leaves one of the four values per quarter of the wave: value 2 * (bit 4) + (bit 5)), the
+// channel bits below by rotations of the row.
+template <int S>
+__device__ __forceinline__ float sum_channels(const float (&v)[4]) {
+    auto swap_add32 = [](float x, float y) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+        return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    };
+    auto swap_add16 = [](float x, float y) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, y), false, false);
+        return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+    };
+    float s = swap_add16(swap_add32(v[0], v[1]), swap_add32(v[2], v[3]));
+    if constexpr (S <= 8) s = dpp_add<0x128>(s);     // row_ror 8
+    if constexpr (S <= 4) s = dpp_add<0x124>(s);     // row_ror 4
+    if constexpr (S <= 2) s = dpp_add<0x122>(s);     // row_ror 2
+    if constexpr (S <= 1) s = dpp_add<0x121>(s);     // row_ror 1
+    return s;
+}
+
+// A wave's place: channels [d0, d0 + nch) of group g of sequence b, steps [t_lo, t_hi) of which [t_lo, tv) exist.
+struct Wave { int b, chunk, tile, g, d0, nch, t_lo, t_hi, tv; };
+
+__device__ __forceinline__ void set_tile(Wave &w, const Plan &pl, int tile_in_group) {
+    w.tile = w.g * pl.tpg + tile_in_group;
+    w.d0 = w.g * pl.Dg + tile_in_group * pl.CH;
+    w.nch = min(pl.CH, pl.Dg - tile_in_group * pl.CH);
+}
+__device__ __forceinline__ void set_time(Wave &w, const Plan &pl, int T, const int32_t *lengths) {
+    w.t_lo = w.chunk * pl.chunk;
+    w.t_hi = min(T, w.t_lo + pl.chunk);
+    w.tv = min(w.t_hi, clamped_length(lengths, w.b, T));
+}
+
+// The decays' exponents per unit of dt, to base 2, of this lane's four states (0 for states that do not exist).
+__device__ __forceinline__ void load_rates(const float *a, int N, const Wave &w, int c, int s, float (&a2)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int n = 4 * s + k;
+        a2[k] = (c < w.nch && n < N) ? a[(long)(w.d0 + c) * N + n] * kLog2e : 0.f;
+    }
+}
+
+// Rows of b or c of one block on their way to LDS: NP values a step (zeros beyond N and behind the end).
+template <typename X, int S>
+struct MapRows {
+    static constexpr int NP = 4 * S;
+    X v[S];
+    __device__ __forceinline__ void load(const void *base, const int64_t *stride, const Wave &w, int N, int t0) {
+        const X *p = static_cast<const X *>(base) + w.b * stride[0] + w.g * stride[2];
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            const int e = lane + 64 * j, t = min(t0 + e / NP, w.tv - 1), n = min(e % NP, N - 1);
+            v[j] = p[(long)t * stride[1] + n];
+        }
+    }
+    __device__ __forceinline__ void store(float *lds, const Wave &w, int N, int t0) const {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < S; ++j) {
+            const int e = lane + 64 * j;
+            lds[e] = (t0 + e / NP < w.tv && e % NP < N) ? to_float(v[j]) : 0.f;
+        }
+    }
+};
+
+// Rows of a (B, T, D) tensor of one block, split over the lanes: element j of a lane is step (lane + 64 j) / CH of the
+// block and channel lane % CH of the wave.
+template <typename X, int S>
+struct Rows {
+    static constexpr int CH = 64 / S, E = Q * CH / 64;
+    X v[E];
+    __device__ __forceinline__ void load(const void *base, const int64_t *stride, const Wave &w, int t0) {
+        const int lane = threadIdx.x & 63;
+        const X *p = static_cast<const X *>(base) + w.b * stride[0] + w.d0 + min(lane % CH, w.nch - 1);
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = p[(long)min(t0 + (lane + 64 * j) / CH, w.tv - 1) * stride[1]];
+    }
+};
+
+// MODE 0: the outputs.  MODE 1: a chunk's end state from a zero start and its sum of dt, for the joining kernel.
+template <typename X, int S, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
+    constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
+    __shared__ float2 s_step[kWaves][Q][CH];                        // dt, dt * u
+    __shared__ __align__(16) float s_b[kWaves][Q][NP], s_c[MODE == 0 ? kWaves : 1][Q][NP];
+    __shared__ float s_y[MODE == 0 ? kWaves : 1][Q][CH];
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long id = (long)blockIdx.x * kWaves + wv;
+    Wave w;
+    const int flat = (int)(id % pl.tiles);
+    const long rest = id / pl.tiles;
+    w.chunk = (int)(rest % pl.nchunks);
+    if (rest / pl.nchunks >= a.B) return;
+    w.b = (int)(rest / pl.nchunks);
+    w.g = flat / pl.tpg;
+    set_tile(w, pl, flat - w.g * pl.tpg);
+    set_time(w, pl, a.T, a.lengths);
+    const int c = lane / S, s = lane % S;
+    const int ec = lane % CH;                                       // this lane's channel when it works per channel
+    const bool e_on = ec < w.nch;
+    const int ed = w.d0 + min(ec, w.nch - 1);
+    const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f;
+    const float skip = (MODE == 0 && a.skip) ? a.skip[ed] : 0.f;
+    float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
+    load_rates(a.a, a.N, w, c, s, a2);
+    if (MODE == 0) {
+        if (pl.nchunks > 1) {
+            const float4 v = reinterpret_cast<const float4 *>(carry)[lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile)];
+            h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
+        } else if (a.initial_state) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c < w.nch && 4 * s + k < a.N) h[k] = a.initial_state[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k];
+        }
+    }
+    Rows<X, S> ru, rd, rz;
+    MapRows<X, S> rb, rc;
+    auto request = [&](int t0) {
+        ru.load(a.u, a.u_stride, w, t0);
+        rd.load(a.delta, a.delta_stride, w, t0);
+        rb.load(a.b, a.b_stride, w, a.N, t0);
+        if (MODE == 0) {
+            rc.load(a.c, a.c_stride, w, a.N, t0);
+            if (a.z) rz.load(a.z, a.z_stride, w, t0);
+        }
+    };
+    if (w.t_lo < w.tv) request(w.t_lo);
+    for (int t0 = w.t_lo; t0 < w.tv; t0 += Q) {
+        float u[E], z[E];
+        wave_sync();
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int et = (lane + 64 * j) / CH;
+            const bool on = e_on && t0 + et < w.tv;
+            u[j] = on ? to_float(ru.v[j]) : 0.f;
+            z[j] = (MODE == 0 && a.z) ? to_float(rz.v[j]) : 0.f;
+            const float raw = to_float(rd.v[j]) + bias;
+            const float dt = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
+            s_step[wv][et][ec] = make_float2(dt, dt * u[j]);
+        }
+        rb.store(&s_b[wv][0][0], w, a.N, t0);
+        if (MODE == 0) rc.store(&s_c[wv][0][0], w, a.N, t0);
+        if (t0 + Q < w.tv) request(t0 + Q);
+        wave_sync();
+        if (MODE == 0 && a.reserve)
+            reinterpret_cast<float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)] = make_float4(h[0], h[1], h[2], h[3]);
+        auto step = [&](int i) {
+            const float2 v = s_step[wv][i][c];
+            const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
+            const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x * a2[k]), h[k], v.y * bb[k]);
+            if (MODE == 1) { dts += v.x; return 0.f; }
+            const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[MODE == 0 ? wv : 0][i][4 * s]);
+            return sum_parts<S>(__builtin_fmaf(c4.x, h[0], __builtin_fmaf(c4.y, h[1], __builtin_fmaf(c4.z, h[2], c4.w * h[3]))));
+        };
+        const int left = w.tv - t0;
+        if (left >= Q) {
+#pragma unroll
+            for (int i = 0; i < Q; i += 4) {
+                float y[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = step(i + r);
+                if (MODE == 1) continue;
+                if constexpr (S >= 4) {              // part r of a channel keeps the sum of step i + r
+                    const float v = s == 0 ? y[0] : s == 1 ? y[1] : s == 2 ? y[2] : y[3];
+                    if (S == 4 || s < 4) s_y[MODE == 0 ? wv : 0][i + s % 4][c] = v;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (s == r % S) s_y[MODE == 0 ? wv : 0][i + r][c] = y[r];
+                }
+            }
+        } else {                                     // the sequence ends inside this block
+            for (int i = 0; i < left; ++i) {
+                const float y = step(i);
+                if (MODE == 0 && s == 0) s_y[MODE == 0 ? wv : 0][i][c] = y;
+            }
+        }
+        if (MODE == 0) {
+            wave_sync();
+            X *yp = static_cast<X *>(a.y) + w.b * a.y_stride[0] + ed;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                const int et = (lane + 64 * j) / CH;
+                if (!e_on || t0 + et >= w.tv) continue;
+                float y = __builtin_fmaf(skip, u[j], s_y[MODE == 0 ? wv : 0][et][ec]);
+                if (a.z) y *= z[j] * sigmoid(z[j]);
+                yp[(long)(t0 + et) * a.y_stride[1]] = from_float<X>(y);
+            }
+        }
+    }
+    if (MODE == 1) {
+        const long at = lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile);
+        reinterpret_cast<float4 *>(carry)[at] = make_float4(h[0], h[1], h[2], h[3]);
+        sdt[at] = dts;
+        return;
+    }
+    X *yp = static_cast<X *>(a.y) + w.b * a.y_stride[0] + ed;
+    for (int t = max(w.t_lo, w.tv) + lane / CH; t < w.t_hi; t += S)
+        if (e_on) yp[(long)t * a.y_stride[1]] = from_float<X>(0.f);
+    if (a.final_state && w.chunk == pl.nchunks - 1 && c < w.nch) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (4 * s + k < a.N) a.final_state[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k] = h[k];
+    }
+}
+
+// Joins the chunks: carry[chunk] becomes what enters the chunk.  `edge`: (B, D, N) entering the first chunk in the
+// order of the pass (the initial state forward, the final state's gradient backward), or null.
+template <int S>
+__global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const float *edge, Plan pl, int D, int N, int backward,
+                                                       float *carry, const float *sdt) {
+    constexpr int CH = 64 / S;
+    const int lane = threadIdx.x, c = lane / S, s = lane % S;
+    Wave w;
+    w.b = blockIdx.x / pl.tiles;
+    const int flat = blockIdx.x - w.b * pl.tiles;
+    w.g = flat / pl.tpg;
+    set_tile(w, pl, flat - w.g * pl.tpg);
+    (void)CH;
+    float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+    load_rates(a, N, w, c, s, a2);
+    if (edge && c < w.nch) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (4 * s + k < N) h[k] = edge[((long)w.b * D + w.d0 + c) * N + 4 * s + k];
+    }
+    constexpr int U = 8;                 // chunks requested together
+    for (int i0 = 0; i0 < pl.nchunks; i0 += U) {
+        float4 v[U];
+        float dt[U];
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            const int i = min(i0 + r, pl.nchunks - 1);
+            const long at = lane_slot(pl, w.b, backward ? pl.nchunks - 1 - i : i, pl.nchunks, w.tile);
+            v[r] = reinterpret_cast<const float4 *>(carry)[at];
+            dt[r] = sdt[at];
+        }
+#pragma unroll
+        for (int r = 0; r < U; ++r) {
+            if (i0 + r >= pl.nchunks) break;
+            const int i = i0 + r;
+            const long at = lane_slot(pl, w.b, backward ? pl.nchunks - 1 - i : i, pl.nchunks, w.tile);
+            reinterpret_cast<float4 *>(carry)[at] = make_float4(h[0], h[1], h[2], h[3]);
+            const float e[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // a chunk without steps passes the state on as it is, also where A is infinite
+                const float p = dt[r] == 0.f ? 1.f : __builtin_amdgcn_exp2f(dt[r] * a2[k]);
+                h[k] = __builtin_fmaf(p, h[k], e[k]);
+            }
+        }
+    }
+}
+
+// Backward.  With g_t the gradient of h_t:  g_t = c_t dy_t + exp(dt_{t+1} A) g_{t+1},
+//     dc_t = sum over channels dy_t h_t            db_t = sum over channels g_t dt_t u_t
+//     du_t = dt_t (g_t . b_t) + skip dy_t          w_t = g_t exp(dt_t A) h_{t-1}
+//     d(dt_t) = u_t (g_t . b_t) + A . w_t          dA = sum over steps dt_t w_t
+// where dy is the gradient in front of the gate.  The four waves of a workgroup are neighbouring waves of one group, one
+// sequence and one chunk: their sums over channels are joined in LDS and one row per workgroup goes to memory.
+// MODE 1 leaves the chunk's gradient at its start from a zero end and its sum of dt.
+template <typename X, int S, int MODE>
+__global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt, float *map_part,
+                                                              float *par_part) {
+    constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
+    __shared__ float4 s_step[kWaves][Q][CH];         // dt, dt * u, dy; then the step's sums g . b, A . w, c . h
+    __shared__ __align__(16) float s_b[kWaves][Q][NP], s_c[kWaves][Q][NP];     // b and c; then the wave's db and dc
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Wave w;
+    int id = blockIdx.x;
+    const int wg = id % pl.wpg;
+    id /= pl.wpg;
+    w.g = id % a.G;
+    id /= a.G;
+    w.chunk = id % pl.nchunks;
+    w.b = id / pl.nchunks;
+    const int in_group = wg * kWaves + wv;
+    const bool wave_on = in_group < pl.tpg;          // the last workgroup of a group may have waves to spare
+    set_tile(w, pl, wave_on ? in_group : pl.tpg - 1);
+    if (!wave_on) w.nch = 0;
+    set_time(w, pl, a.T, a.lengths);
+    if (MODE == 1 && !wave_on) return;
+    Wave from = w;                                   // where a spare wave loads from (nothing is used)
+    if (!wave_on) from.nch = 1;
+    const int c = lane / S, s = lane % S, ec = lane % CH;
+    const bool e_on = ec < w.nch;
+    const int ed = w.d0 + min(ec, from.nch - 1);
+    const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f;
+    const float skip = (MODE == 0 && a.skip) ? a.skip[ed] : 0.f;
+    float a2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
+    load_rates(a.a, a.N, w, c, s, a2);
+    if (MODE == 0) {
+        if (pl.nchunks > 1) {
+            if (wave_on) {
+                const float4 v = reinterpret_cast<const float4 *>(carry)[lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile)];
+                g[0] = v.x; g[1] = v.y; g[2] = v.z; g[3] = v.w;
+            }
+        } else if (a.dfinal) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c < w.nch && 4 * s + k < a.N) g[k] = a.dfinal[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k];
+        }
+    }
+    Rows<X, S> ru, rd, rz, rg;
+    MapRows<X, S> rb, rc;
+    float4 rh;
+    auto request = [&](int t0) {
+        rd.load(a.delta, a.delta_stride, from, t0);
+        if (a.dy) rg.load(a.dy, a.dy_stride, from, t0);
+        rc.load(a.c, a.c_stride, from, a.N, t0);
+        if (a.z) rz.load(a.z, a.z_stride, from, t0);
+        if (MODE == 0) {
+            ru.load(a.u, a.u_stride, from, t0);
+            rb.load(a.b, a.b_stride, from, a.N, t0);
+            rh = reinterpret_cast<const float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)];
+        }
+    };
+    // sums over all steps: dA by state, dskip and ddelta_bias by channel
+    float dA[4] = {0.f, 0.f, 0.f, 0.f}, dskip = 0.f, dbias = 0.f;
+    const int last = w.tv > w.t_lo ? w.t_lo + (w.tv - 1 - w.t_lo) / Q * Q : w.t_lo - Q;
+    if (last >= w.t_lo) request(last);
+    for (int t0 = last; t0 >= w.t_lo; t0 -= Q) {
+        float u[E], z[E], out[E], dt[E], dy[E], slope[E];
+        wave_sync();
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int et = (lane + 64 * j) / CH;
+            const bool on = e_on && t0 + et < w.tv;
+            u[j] = (MODE == 0 && on) ? to_float(ru.v[j]) : 0.f;
+            z[j] = a.z ? to_float(rz.v[j]) : 0.f;
+            out[j] = (a.dy && on) ? to_float(rg.v[j]) : 0.f;
+            const float raw = to_float(rd.v[j]) + bias;
+            dt[j] = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
+            slope[j] = a.softplus ? sigmoid(raw) : 1.f;
+            dy[j] = (a.z && on) ? out[j] * z[j] * sigmoid(z[j]) : out[j];
+            s_step[wv][et][ec] = make_float4(dt[j], dt[j] * u[j], dy[j], 0.f);
+        }
+        if (MODE == 0) rb.store(&s_b[wv][0][0], w, a.N, t0);
+        rc.store(&s_c[wv][0][0], w, a.N, t0);
+        const float h0[4] = {rh.x, rh.y, rh.z, rh.w};
+        if (t0 > w.t_lo) request(t0 - Q);
+        wave_sync();
+        const int left = w.tv - t0;                  // steps of this block that exist (Q or more: all)
+        if (MODE == 1) {
+            for (int i = min(left, Q) - 1; i >= 0; --i) {
+                const float4 v = s_step[wv][i][c];
+                const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
+                const float cc[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) g[k] = __builtin_amdgcn_exp2f(v.x * a2[k]) * __builtin_fmaf(v.z, cc[k], g[k]);
+                dts += v.x;
+            }
+            continue;
+        }
+        float blkA[4] = {0.f, 0.f, 0.f, 0.f};
+        auto block = [&](auto whole) {
+            float decay[Q][4], h[Q][4];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) {
+                if (!whole.value && i >= left) continue;
+                const float4 v = s_step[wv][i][c];
+                const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
+                const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    decay[i][k] = __builtin_amdgcn_exp2f(v.x * a2[k]);
+                    h[i][k] = __builtin_fmaf(decay[i][k], i ? h[i ? i - 1 : 0][k] : h0[k], v.y * bb[k]);
+                }
+            }
+#pragma unroll
+            for (int i = Q - 1; i >= 0; --i) {
+                if (!whole.value && i >= left) continue;
+                const float4 v = s_step[wv][i][c];
+                const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
+                const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
+                const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
+                float db[4], dc[4], gb = 0.f, aw = 0.f, ch = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float gt = __builtin_fmaf(v.z, cc[k], g[k]);
+                    dc[k] = v.z * h[i][k];
+                    db[k] = v.y * gt;
+                    gb = __builtin_fmaf(gt, bb[k], gb);
+                    ch = __builtin_fmaf(cc[k], h[i][k], ch);
+                    g[k] = gt * decay[i][k];
+                    const float wk = g[k] * (i ? h[i ? i - 1 : 0][k] : h0[k]);
+                    aw = __builtin_fmaf(wk, a2[k], aw);
+                    blkA[k] = __builtin_fmaf(wk, v.x, blkA[k]);
+                }
+                gb = sum_parts<S>(gb);
+                aw = sum_parts<S>(aw);
+                if (a.z) ch = sum_parts<S>(ch);
+                const float sb = sum_channels<S>(db), sc = sum_channels<S>(dc);
+                if (s == 0) s_step[wv][i][c] = make_float4(gb, aw, ch, 0.f);
+                // lane (quarter q, part s) has the sums of state 4 s + value of quarter q
+                if (lane % 16 < S) {
+                    const int n = 4 * s + 2 * ((lane >> 4) & 1) + (lane >> 5);
+                    s_b[wv][i][n] = sb;
+                    s_c[wv][i][n] = sc;
+                }
+            }
+        };
+        if (left >= Q) block(std::true_type{});
+        else block(std::false_type{});
+#pragma unroll
+        for (int k = 0; k < 4; ++k) dA[k] += blkA[k];
+        wave_sync();
+        float bs = 0.f, bb = 0.f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const int et = (lane + 64 * j) / CH;
+            if (!e_on || t0 + et >= w.tv) continue;
+            const float4 r = s_step[wv][et][ec];
+            const long t = t0 + et;
+            const float du = __builtin_fmaf(r.x, dt[j], skip * dy[j]);
+            const float dd = __builtin_fmaf(r.x, u[j], kLn2 * r.y) * slope[j];
+            bs = __builtin_fmaf(dy[j], u[j], bs);
+            bb += dd;
+            if (a.du) static_cast<X *>(a.du)[w.b * a.du_stride[0] + t * a.du_stride[1] + ed] = from_float<X>(du);
+            if (a.ddelta) static_cast<X *>(a.ddelta)[w.b * a.ddelta_stride[0] + t * a.ddelta_stride[1] + ed] = from_float<X>(dd);
+            if (a.dz) {
+                const float sg = sigmoid(z[j]);
+                const float v = out[j] * __builtin_fmaf(skip, u[j], r.z) * sg * __builtin_fmaf(z[j], 1.f - sg, 1.f);
+                static_cast<X *>(a.dz)[w.b * a.dz_stride[0] + t * a.dz_stride[1] + ed] = from_float<X>(v);
+            }
+        }
+        dskip += bs;
+        dbias += bb;
+        if (map_part) {
+            // the four waves' sums of this block, joined: map_part[b][g][workgroup][t][db, dc][NP]
+            __syncthreads();
+            float *to = map_part + ((((long)w.b * a.G + w.g) * pl.wpg + wg) * a.T + t0) * 2 * NP;
+            for (int e = threadIdx.x; e < 2 * Q * NP; e += 64 * kWaves) {
+                const int t = e / (2 * NP), n = e % (2 * NP);
+                if (t0 + t >= w.tv) break;
+                float v = 0.f;
+#pragma unroll
+                for (int q = 0; q < kWaves; ++q) v += n < NP ? s_b[q][t][n] : s_c[q][t][n - NP];
+                to[e] = v;
+            }
+            __syncthreads();
+        }
+    }
+    if (MODE == 1) {
+        const long at = lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile);
+        reinterpret_cast<float4 *>(carry)[at] = make_float4(g[0], g[1], g[2], g[3]);
+        sdt[at] = dts;
+        return;
+    }
+    // rows behind the end
+    for (int t = max(w.t_lo, w.tv) + lane / CH; t < w.t_hi; t += S) {
+        if (!e_on) break;
+        const X zero = from_float<X>(0.f);
+        if (a.du) static_cast<X *>(a.du)[w.b * a.du_stride[0] + t * a.du_stride[1] + ed] = zero;
+        if (a.ddelta) static_cast<X *>(a.ddelta)[w.b * a.ddelta_stride[0] + t * a.ddelta_stride[1] + ed] = zero;
+        if (a.dz) static_cast<X *>(a.dz)[w.b * a.dz_stride[0] + t * a.dz_stride[1] + ed] = zero;
+    }
+    if (a.dinitial && w.chunk == 0 && c < w.nch) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (4 * s + k < a.N) a.dinitial[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k] = g[k];
+    }
+    if (!par_part) return;
+    // par_part[b, chunk][dA (D, N) | dskip (D) | ddelta_bias (D)]
+    float *to = par_part + ((long)w.b * pl.nchunks + w.chunk) * a.D * (a.N + 2);
+    if (c < w.nch) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (4 * s + k < a.N) to[(long)(w.d0 + c) * a.N + 4 * s + k] = dA[k];
+    }
+#pragma unroll
+    for (int m = CH; m < 64; m <<= 1) {
+        dskip += __shfl_xor(dskip, m);
+        dbias += __shfl_xor(dbias, m);
+    }
+    if (lane < CH && e_on) {
+        to[(long)a.D * a.N + ed] = dskip;
+        to[(long)a.D * (a.N + 1) + ed] = dbias;
+    }
+}
+
+// db, dc (B, T, G, N) from map_part[b][g][workgroup][t][db, dc][NP], the workgroups in order; zeros behind the end.
+template <typename X>
+__global__ __launch_bounds__(256) void scan_map_grad_kernel(tgru_scan_args a, Plan pl, const float *__restrict__ map_part) {
+    const int NP = 4 * pl.S;
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;         // (b, g, t, db | dc, n)
+    const int e = (int)(id % (2 * NP));
+    const long row = id / (2 * NP);
+    const int t = (int)(row % a.T);
+    const long bg = row / a.T;
+    const int n = e % NP;
+    if (bg >= (long)a.B * a.G || n >= a.N) return;
+    const int b = (int)(bg / a.G), g = (int)(bg % a.G);
+    float v = 0.f;
+    if (t < clamped_length(a.lengths, b, a.T)) {
+        const float *p = map_part + (bg * pl.wpg * a.T + t) * 2 * NP + e;
+        const long step = (long)a.T * 2 * NP;
+        for (int q = 0; q < pl.wpg; ++q) v += p[q * step];
+    }
+    X *to = static_cast<X *>(e < NP ? a.db : a.dc);
+    if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
+}
+
+// da, dskip, ddelta_bias from par_part[rows][D (N + 2)]: 64 columns x 4 groups of rows per workgroup, joined in order.
+__global__ __launch_bounds__(256) void scan_param_grad_kernel(const float *__restrict__ part, int rows, int D, int N, float *da,
+                                                              float *dskip, float *dbias) {
+    __shared__ float red[4][64];
+    const int c = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    const long cols = (long)D * (N + 2), col = (long)blockIdx.x * 64 + c;
+    const int per = (rows + 3) / 4, r0 = grp * per, r1 = min(rows, r0 + per);
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col < cols) {
+        int r = r0;
+        for (; r + 3 < r1; r += 4)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[q] += part[(long)(r + q) * cols + col];
+        for (; r < r1; ++r) s[0] += part[(long)r * cols + col];
+    }
+    red[grp][c] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (grp != 0 || col >= cols) return;
+    const float v = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+    const long dn = (long)D * N;
+    if (col < dn) { if (da) da[col] = v; }
+    else if (col < dn + D) { if (dskip) dskip[col - dn] = v; }
+    else if (dbias) dbias[col - dn - D] = v;
+}
+
+// One token: a wave takes CH channels of one row.  Rows with one slot are taken in order by the first one's wave.
+template <typename X, int S>
+__global__ __launch_bounds__(64) void scan_step_kernel(tgru_scan_step_args a, int tpg, int tiles) {
+    constexpr int CH = 64 / S;
+    const int lane = threadIdx.x, c = lane / S, s = lane % S;
+    const int row0 = blockIdx.x / tiles, flat = blockIdx.x - row0 * tiles;
+    const int grp = flat / tpg, Dg = a.D / a.G, first = (flat - grp * tpg) * CH;
+    const bool on = c < Dg - first;
+    const int d = grp * Dg + first + (on ? c : 0);
+    const int slot = a.slots ? __builtin_amdgcn_readfirstlane(a.slots[row0]) : row0;
+    if (slot < 0 || slot >= a.P) {
+        if (on && s == 0) static_cast<X *>(a.y)[row0 * a.y_stride + d] = from_float<X>(0.f);
+        return;
+    }
+    if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
+    float h[4], a2[4];
+    const long so = ((long)slot * a.D + d) * a.N + 4 * s;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const bool has = 4 * s + k < a.N;
+        const long at = has ? k : -4 * s;             // a state that does not exist reads the channel's first one
+        h[k] = has ? a.state[so + at] : 0.f;
+        a2[k] = has ? a.a[(long)d * a.N + 4 * s + k] * kLog2e : 0.f;
+    }
+    const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+    for (int row = row0; row < a.B;) {
+        const float u = to_float(static_cast<const X *>(a.u)[row * a.u_stride + d]);
+        const float raw = to_float(static_cast<const X *>(a.delta)[row * a.delta_stride + d]) + bias;
+        const float dt = a.softplus ? softplus(raw) : raw;
+        const X *b = static_cast<const X *>(a.b) + row * a.b_stride[0] + grp * a.b_stride[1];
+        const X *m = static_cast<const X *>(a.c) + row * a.c_stride[0] + grp * a.c_stride[1];
+        float y = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int n = min(4 * s + k, a.N - 1);
+            const float bb = 4 * s + k < a.N ? to_float(b[n]) : 0.f, cc = 4 * s + k < a.N ? to_float(m[n]) : 0.f;
+            h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a2[k]), h[k], dt * u * bb);
+            y = __builtin_fmaf(cc, h[k], y);
+        }
+        y = __builtin_fmaf(skip, u, sum_parts<S>(y));
+        if (a.z) {
+            const float z = to_float(static_cast<const X *>(a.z)[row * a.z_stride + d]);
+            y *= z * sigmoid(z);
+        }
+        if (on && s == 0) static_cast<X *>(a.y)[row * a.y_stride + d] = from_float<X>(y);
+        if (!a.slots) break;
+        row = find_slot(a.slots, row + 1, a.B, slot);
+    }
+    if (!on) return;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (4 * s + k < a.N) a.state_out[so + k] = h[k];
+}
+
+int lanes_per_channel(int N) {
+    int S = 1;
+    while (4 * S < N) S <<= 1;
+    return S;
+}
+
+// Chunks of time: as many as fill the chip, none where the channels alone do.
+Plan make_plan(int B, int T, int D, int N, int G) {
+    Plan p;
+    p.S = lanes_per_channel(N);
+    p.CH = 64 / p.S;
+    p.Dg = D / G;
+    p.tpg = (p.Dg + p.CH - 1) / p.CH;
+    p.tiles = p.tpg * G;
+    p.wpg = (p.tpg + kWaves - 1) / kWaves;
+    p.nblk = (T + Q - 1) / Q;
+    p.nchunks = 1;
+    const long waves = (long)B * p.tiles;
+    if (waves < 768) {
+        const long want = (2048 + waves - 1) / waves, most = (p.nblk + 3) / 4;      // four blocks a chunk at least
+        const long n = want < most ? want : most;
+        if (n >= 3) p.nchunks = (int)n;                 // a chunked pass does the work twice
+    }
+    p.chunk = (p.nblk + p.nchunks - 1) / p.nchunks * Q;
+    p.nchunks = (T + p.chunk - 1) / p.chunk;
+    return p;
+}
+
+int scan_dims(int B, int T, int D, int N, int G) {
+    if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || N > TGRU_SCAN_MAX_STATES || D % G) return TGRU_E_DIMS;
+    if (T > (1 << 30) || D > (1 << 26)) return TGRU_E_DIMS;
+    const Plan p = make_plan(B, T, D, N, G);
+    // workgroup numbers of the widest launch (the maps' gradients: one thread per (b, t, g, db | dc, state)) in 31 bits
+    if ((double)B * p.tiles * p.nchunks >= 2147483648.0 || (double)B * T * G * 8 * p.S / 256 >= 2147483647.0) return TGRU_E_DIMS;
+    return TGRU_OK;
+}
+
+struct Workspace { size_t carry, sdt, map, par, total; };       // offsets in floats
+Workspace workspace_of(const Plan &p, int B, int T, int D, int N, int G, bool backward) {
+    Workspace w;
+    size_t off = 0;
+    const size_t lanes = p.nchunks > 1 ? (size_t)B * p.nchunks * p.tiles * 64 : 0;
+    w.carry = off; off += 4 * lanes;
+    w.sdt = off; off += lanes;
+    w.map = off; off += backward ? (size_t)B * G * p.wpg * T * 8 * p.S : 0;
+    w.par = off; off += backward ? (size_t)B * p.nchunks * D * (N + 2) : 0;
+    w.total = off;
+    return w;
+}
+
+#define TGRU_DONE() do { if (hipGetLastError() != hipSuccess) return TGRU_E_LAUNCH; } while (0)
+
+template <typename X, int S>
+int run_scan(const tgru_scan_args &a, const Plan &pl, bool backward, hipStream_t s) {
+    const Workspace ws = workspace_of(pl, a.B, a.T, a.D, a.N, a.G, backward);
+    float *carry = a.workspace + ws.carry, *sdt = a.workspace + ws.sdt;
+    const dim3 join((unsigned)(a.B * pl.tiles)), block(64 * kWaves);
+    if (!backward) {
+        const dim3 grid((unsigned)(((long)a.B * pl.nchunks * pl.tiles + kWaves - 1) / kWaves));
+        if (pl.nchunks > 1) {
+            TGRU_LAUNCH((scan_fwd_kernel<X, S, 1>), grid, block, 0, s, a, pl, carry, sdt);
+            TGRU_DONE();
+            TGRU_LAUNCH((scan_join_kernel<S>), join, dim3(64), 0, s, a.a, a.initial_state, pl, a.D, a.N, 0, carry, sdt);
+            TGRU_DONE();
+        }
+        TGRU_LAUNCH((scan_fwd_kernel<X, S, 0>), grid, block, 0, s, a, pl, carry, sdt);
+        TGRU_DONE();
+        return TGRU_OK;
+    }
+    const dim3 grid((unsigned)((long)a.B * pl.nchunks * a.G * pl.wpg));
+    float *map = (a.db || a.dc) ? a.workspace + ws.map : nullptr;
+    float *par = (a.da || a.dskip || a.ddelta_bias) ? a.workspace + ws.par : nullptr;
+    if (pl.nchunks > 1) {
+        TGRU_LAUNCH((scan_bwd_kernel<X, S, 1>), grid, block, 0, s, a, pl, carry, sdt, nullptr, nullptr);
+        TGRU_DONE();
+        TGRU_LAUNCH((scan_join_kernel<S>), join, dim3(64), 0, s, a.a, a.dfinal, pl, a.D, a.N, 1, carry, sdt);
+        TGRU_DONE();
+    }
+    TGRU_LAUNCH((scan_bwd_kernel<X, S, 0>), grid, block, 0, s, a, pl, carry, sdt, map, par);
+    TGRU_DONE();
+    if (map) {
+        const long n = (long)a.B * a.G * a.T * 8 * S;
+        TGRU_LAUNCH((scan_map_grad_kernel<X>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, pl, map);
+        TGRU_DONE();
+    }
+    if (par) {
+        const long cols = (long)a.D * (a.N + 2);
+        TGRU_LAUNCH(scan_param_grad_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s, par, a.B * pl.nchunks, a.D, a.N,
+                    a.da, a.dskip, a.ddelta_bias);
+        TGRU_DONE();
+    }
+    return TGRU_OK;
+}
+
+template <typename X>
+int run_scan_lanes(const tgru_scan_args &a, const Plan &pl, bool backward, hipStream_t s) {
+    switch (pl.S) {
+    case 1: return run_scan<X, 1>(a, pl, backward, s);
+    case 2: return run_scan<X, 2>(a, pl, backward, s);
+    case 4: return run_scan<X, 4>(a, pl, backward, s);
+    case 8: return run_scan<X, 8>(a, pl, backward, s);
+    default: return run_scan<X, 16>(a, pl, backward, s);
+    }
+}
+
+int scan_call(const tgru_scan_args *a, bool backward, hipStream_t s) {
+    if (!a) return TGRU_E_NULL;
+    if (int rc = scan_dims(a->B, a->T, a->D, a->N, a->G)) return rc;
+    if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
+    if (!a->u || !a->delta || !a->b || !a->c || !a->a) return TGRU_E_NULL;
+    const Plan pl = make_plan(a->B, a->T, a->D, a->N, a->G);
+    if (backward ? !a->reserve || (a->dz && !a->z) : !a->y) return TGRU_E_NULL;
+    if ((backward || pl.nchunks > 1) && !a->workspace) return TGRU_E_NULL;
+    if (((uintptr_t)a->reserve & 15) || ((uintptr_t)a->workspace & 15)) return TGRU_E_ALIGN;
+    if (int rc = check_device()) return rc;
+    if (a->dtype == TGRU_DTYPE_F32) return run_scan_lanes<float>(*a, pl, backward, s);
+    if (a->dtype == TGRU_DTYPE_BF16) return run_scan_lanes<__bf16>(*a, pl, backward, s);
+    return run_scan_lanes<_Float16>(*a, pl, backward, s);
+}
+
+template <typename X, int S>
+int run_scan_step(const tgru_scan_step_args &a, hipStream_t s) {
+    const int CH = 64 / S, tpg = (a.D / a.G + CH - 1) / CH, tiles = tpg * a.G;
+    TGRU_LAUNCH((scan_step_kernel<X, S>), dim3((unsigned)((long)a.B * tiles)), dim3(64), 0, s, a, tpg, tiles);
+    TGRU_DONE();
+    return TGRU_OK;
+}
+
+template <typename X>
+int run_scan_step_lanes(const tgru_scan_step_args &a, hipStream_t s) {
+    switch (lanes_per_channel(a.N)) {
+    case 1: return run_scan_step<X, 1>(a, s);
+    case 2: return run_scan_step<X, 2>(a, s);
+    case 4: return run_scan_step<X, 4>(a, s);
+    case 8: return run_scan_step<X, 8>(a, s);
+    default: return run_scan_step<X, 16>(a, s);
+    }
+}
+
+}  // namespace ssm
+}  // namespace tgru
+
+using namespace tgru::ssm;
+
+extern "C" {
+
+size_t tgru_scan_reserve_bytes(int B, int T, int D, int N, int G) {
+    if (scan_dims(B, T, D, N, G) != TGRU_OK) return 0;
+    const Plan p = make_plan(B, T, D, N, G);
+    return (size_t)B * p.nblk * p.tiles * 64 * 4 * sizeof(float);
+}
+
+size_t tgru_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward) {
+    if (scan_dims(B, T, D, N, G) != TGRU_OK) return 0;
+    const Plan p = make_plan(B, T, D, N, G);
+    return workspace_of(p, B, T, D, N, G, backward != 0).total * sizeof(float);
+}
+
+int tgru_scan_forward(const tgru_scan_args *a, tgru_stream_t stream) { return scan_call(a, false, (hipStream_t)stream); }
+int tgru_scan_backward(const tgru_scan_args *a, tgru_stream_t stream) { return scan_call(a, true, (hipStream_t)stream); }
+
+int tgru_scan_step(const tgru_scan_step_args *a, tgru_stream_t stream) {
+    if (!a) return TGRU_E_NULL;
+    if (a->B <= 0 || a->P <= 0 || a->D <= 0 || a->N <= 0 || a->G <= 0 || a->N > TGRU_SCAN_MAX_STATES || a->D % a->G) return TGRU_E_DIMS;
+    if ((!a->slots && a->P < a->B) || (double)a->B * a->D >= 2147483648.0) return TGRU_E_DIMS;
+    if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
+    if (!a->u || !a->delta || !a->b || !a->c || !a->a || !a->state || !a->state_out || !a->y) return TGRU_E_NULL;
+    if (int rc = tgru::check_device()) return rc;
+    if (a->dtype == TGRU_DTYPE_F32) return run_scan_step_lanes<float>(*a, (hipStream_t)stream);
+    if (a->dtype == TGRU_DTYPE_BF16) return run_scan_step_lanes<__bf16>(*a, (hipStream_t)stream);
+    return run_scan_step_lanes<_Float16>(*a, (hipStream_t)stream);
+}
+
+}  // extern "C"

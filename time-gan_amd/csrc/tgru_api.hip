@@ -137,6 +137,12 @@ int device_ok() {
     return k == 1 ? TGRU_OK : TGRU_E_NOGPU;
 }
 
+}  // namespace
+
+int tgru::check_device() { return device_ok(); }
+
+namespace {
+
 // reserve: [L x 4 gate planes][(L-1) intermediate outputs][top output if layout != TBF]
 size_t reserve_floats(const Dims &d) {
     size_t n = (size_t)d.L * 4 * align64(d.TBH());
@@ -281,6 +287,7 @@ const char *tgru_error_string(int code) {
     case TGRU_E_NOGPU: return "the current device is not a gfx950 GPU";
     case TGRU_E_TOOBIG: return "the call needs more scratch memory than tgru_forward_static holds "
                                "(TGRU_STATIC_WORKSPACE_BYTES); use tgru_forward with a workspace";
+    case TGRU_E_DTYPE: return "unknown element type (TGRU_DTYPE_F32, _BF16 or _F16)";
     default: return "unknown error";
     }
 }

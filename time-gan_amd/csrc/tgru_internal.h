@@ -28,6 +28,9 @@ struct Switches {
 };
 Switches &switches();
 
+// TGRU_OK if the current device is a gfx950 GPU, else TGRU_E_NOGPU (looked up once per device).
+int check_device();
+
 // ----------------------------------------------------------------------------------------------
 // Row addressing.  Inside the library every per-(b,t) buffer is time-major: row = t*B + b.
 // A RowMap turns such an internal row into the row of a caller tensor in its layout, or -1

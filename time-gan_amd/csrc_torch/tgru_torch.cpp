@@ -176,9 +176,12 @@ std::vector<Tensor> gru_apply(const Tensor &x, const c10::optional<Tensor> &h0, 
 
 }  // namespace
 
+void bind_ssm(py::module_ &m);      // ssm_torch.cpp: the state-space operators
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "C++ autograd binding of the tgru GRU (include/tgru.h) for eager callers";
     m.def("gru_apply", &gru_apply, "differentiable multi-layer GRU: (x, h0, lengths, toff, B, T, layout, weights) -> (y, h_n)",
           py::arg("x"), py::arg("h0"), py::arg("lengths"), py::arg("toff"), py::arg("B"), py::arg("T"), py::arg("layout"),
           py::arg("weights"));
+    bind_ssm(m);
 }
