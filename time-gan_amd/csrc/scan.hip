@@ -32,6 +32,7 @@ namespace ssm {
 
 constexpr int Q = 16;                // steps per block
 constexpr int kWaves = 4;            // per workgroup
+constexpr int64_t kMaxRowStride = TGRU_SCAN_MAX_ROW_STRIDE;
 
 struct Plan {                        // how a call is cut up; made on the host
     int S, CH;                       // lanes per channel, channels per wave
@@ -111,43 +112,99 @@ __device__ __forceinline__ void load_rates(const float *a, int N, const Wave &w,
     }
 }
 
-// Rows of b or c of one block on their way to LDS: NP values a step (zeros beyond N and behind the end).
-template <typename X, int S>
-struct MapRows {
-    static constexpr int NP = 4 * S;
-    X v[S];
-    __device__ __forceinline__ void load(const void *base, const int64_t *stride, const Wave &w, int N, int t0) {
-        const X *p = static_cast<const X *>(base) + w.b * stride[0] + w.g * stride[2];
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const int e = lane + 64 * j, t = min(t0 + e / NP, w.tv - 1), n = min(e % NP, N - 1);
-            v[j] = p[(long)t * stride[1] + n];
-        }
-    }
-    __device__ __forceinline__ void store(float *lds, const Wave &w, int N, int t0) const {
-        const int lane = threadIdx.x & 63;
-#pragma unroll
-        for (int j = 0; j < S; ++j) {
-            const int e = lane + 64 * j;
-            lds[e] = (t0 + e / NP < w.tv && e % NP < N) ? to_float(v[j]) : 0.f;
-        }
-    }
-};
+// Rows of a tensor of one block, split over the lanes.  All addresses are a base that is the same for the whole wave (and
+// moves by whole blocks) plus a 32-bit byte offset of the lane, so a load costs no vector arithmetic; row strides are below
+// 2^26 elements for that (kMaxRowStride).  Only a block in which the sequence ends has to hold every lane back from the
+// rows behind the end.
 
-// Rows of a (B, T, D) tensor of one block, split over the lanes: element j of a lane is step (lane + 64 j) / CH of the
-// block and channel lane % CH of the wave.
+// A (B, T, D) tensor: element j of a lane is step lane / CH + j S of the block, channel lane % CH of the wave.
 template <typename X, int S>
 struct Rows {
     static constexpr int CH = 64 / S, E = Q * CH / 64;
-    X v[E];
-    __device__ __forceinline__ void load(const void *base, const int64_t *stride, const Wave &w, int t0) {
+    const char *base;                // step 0 of the wave's channels
+    long row;                        // bytes from step to step
+    unsigned lane_off, col;
+    __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int d0, int nch) {
         const int lane = threadIdx.x & 63;
-        const X *p = static_cast<const X *>(base) + w.b * stride[0] + w.d0 + min(lane % CH, w.nch - 1);
+        base = reinterpret_cast<const char *>(static_cast<const X *>(p) + b * stride[0] + d0);
+        row = stride[1] * (long)sizeof(X);
+        col = min(lane % CH, nch - 1) * (unsigned)sizeof(X);
+        lane_off = (unsigned)(lane / CH) * (unsigned)row + col;
+    }
+    // rows t0 .. t0 + Q - 1 of which `left` exist
+    __device__ __forceinline__ void load(X (&v)[E], int t0, int left) const {
+        const char *p = base + t0 * row;
+        if (left >= Q) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = p[(long)min(t0 + (lane + 64 * j) / CH, w.tv - 1) * stride[1]];
+            for (int j = 0; j < E; ++j, p += S * row) v[j] = *reinterpret_cast<const X *>(p + lane_off);
+        } else {
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                v[j] = *reinterpret_cast<const X *>(p + ((unsigned)min((int)(threadIdx.x & 63) / CH + j * S, left - 1) * (unsigned)row + col));
+        }
+    }
+    __device__ __forceinline__ void store(int t0, int j, float v) const {
+        *reinterpret_cast<X *>(const_cast<char *>(base) + (t0 + j * S) * row + lane_off) = from_float<X>(v);
     }
 };
+
+// b or c: NP = 4 S values a step (zeros beyond N and behind the end), element j of a lane is value lane % NP of step
+// lane / NP + j 64 / NP.
+template <typename X, int S>
+struct Maps {
+    static constexpr int NP = 4 * S, RPJ = 64 / NP;
+    const char *base;
+    long row;
+    unsigned lane_off, col;
+    __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int g, int N) {
+        const int lane = threadIdx.x & 63;
+        base = reinterpret_cast<const char *>(static_cast<const X *>(p) + b * stride[0] + g * stride[2]);
+        row = stride[1] * (long)sizeof(X);
+        col = min(lane % NP, N - 1) * (unsigned)sizeof(X);
+        lane_off = (unsigned)(lane / NP) * (unsigned)row + col;
+    }
+    __device__ __forceinline__ void load(X (&v)[S], int t0, int left) const {
+        const char *p = base + t0 * row;
+        if (left >= Q) {
+#pragma unroll
+            for (int j = 0; j < S; ++j, p += RPJ * row) v[j] = *reinterpret_cast<const X *>(p + lane_off);
+        } else {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                v[j] = *reinterpret_cast<const X *>(p + ((unsigned)min((int)(threadIdx.x & 63) / NP + j * RPJ, left - 1) * (unsigned)row + col));
+        }
+    }
+    __device__ __forceinline__ static void to_lds(float *lds, const X (&v)[S], int N, int left) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int j = 0; j < S; ++j)
+            lds[lane + 64 * j] = (lane / NP + j * RPJ < left && lane % NP < N) ? to_float(v[j]) : 0.f;
+    }
+};
+
+// x, kept where it is: the compiler may not move the computation of x into a branch behind this point.
+__device__ __forceinline__ float pin(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// Writes four steps' values, which all lanes of a channel (or all replicas of a sum) hold, with one write per lane that
+// stores step `which` of 0..3; lanes beyond the first four repeat a value.  `n` replicas: fewer than four write several.
+template <int n, typename F>
+__device__ __forceinline__ void write_four(int replica, F &&write) {
+    if constexpr (n >= 4) {
+        write(replica & 3, [&](const float (&v)[4]) {
+            const float lo = (replica & 1) ? v[1] : v[0], hi = (replica & 1) ? v[3] : v[2];
+            return (replica & 2) ? hi : lo;
+        });
+    } else if constexpr (n == 2) {
+        write(replica, [&](const float (&v)[4]) { return replica ? v[1] : v[0]; });
+        write(2 + replica, [&](const float (&v)[4]) { return replica ? v[3] : v[2]; });
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) write(r, [&](const float (&v)[4]) { return v[r]; });
+    }
+}
 
 // MODE 0: the outputs.  MODE 1: a chunk's end state from a zero start and its sum of dt, for the joining kernel.
 template <typename X, int S, int MODE>
@@ -185,34 +242,45 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
                 if (c < w.nch && 4 * s + k < a.N) h[k] = a.initial_state[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k];
         }
     }
-    Rows<X, S> ru, rd, rz;
-    MapRows<X, S> rb, rc;
+    Rows<X, S> pu, pd, pz, py;
+    Maps<X, S> pb, pc;
+    pu.init(a.u, a.u_stride, w.b, w.d0, w.nch);
+    pd.init(a.delta, a.delta_stride, w.b, w.d0, w.nch);
+    pb.init(a.b, a.b_stride, w.b, w.g, a.N);
+    if (MODE == 0) {
+        py.init(a.y, a.y_stride, w.b, w.d0, w.nch);
+        pc.init(a.c, a.c_stride, w.b, w.g, a.N);
+        if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, w.nch);
+    }
+    X ru[E], rd[E], rz[E], rb[S], rc[S];
     auto request = [&](int t0) {
-        ru.load(a.u, a.u_stride, w, t0);
-        rd.load(a.delta, a.delta_stride, w, t0);
-        rb.load(a.b, a.b_stride, w, a.N, t0);
+        const int left = w.tv - t0;
+        pu.load(ru, t0, left);
+        pd.load(rd, t0, left);
+        pb.load(rb, t0, left);
         if (MODE == 0) {
-            rc.load(a.c, a.c_stride, w, a.N, t0);
-            if (a.z) rz.load(a.z, a.z_stride, w, t0);
+            pc.load(rc, t0, left);
+            if (a.z) pz.load(rz, t0, left);
         }
     };
     if (w.t_lo < w.tv) request(w.t_lo);
     for (int t0 = w.t_lo; t0 < w.tv; t0 += Q) {
         float u[E], z[E];
+        const int left = w.tv - t0;
         wave_sync();
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            const int et = (lane + 64 * j) / CH;
-            const bool on = e_on && t0 + et < w.tv;
-            u[j] = on ? to_float(ru.v[j]) : 0.f;
-            z[j] = (MODE == 0 && a.z) ? to_float(rz.v[j]) : 0.f;
-            const float raw = to_float(rd.v[j]) + bias;
+            const int et = lane / CH + j * S;
+            const bool on = e_on && et < left;
+            u[j] = on ? to_float(ru[j]) : 0.f;
+            z[j] = (MODE == 0 && a.z) ? to_float(rz[j]) : 0.f;
+            const float raw = to_float(rd[j]) + bias;
             const float dt = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
             s_step[wv][et][ec] = make_float2(dt, dt * u[j]);
         }
-        rb.store(&s_b[wv][0][0], w, a.N, t0);
-        if (MODE == 0) rc.store(&s_c[wv][0][0], w, a.N, t0);
-        if (t0 + Q < w.tv) request(t0 + Q);
+        pb.to_lds(&s_b[wv][0][0], rb, a.N, left);
+        if (MODE == 0) pc.to_lds(&s_c[wv][0][0], rc, a.N, left);
+        if (left > Q) request(t0 + Q);
         wave_sync();
         if (MODE == 0 && a.reserve)
             reinterpret_cast<float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)] = make_float4(h[0], h[1], h[2], h[3]);
@@ -227,7 +295,6 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
             const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[MODE == 0 ? wv : 0][i][4 * s]);
             return sum_parts<S>(__builtin_fmaf(c4.x, h[0], __builtin_fmaf(c4.y, h[1], __builtin_fmaf(c4.z, h[2], c4.w * h[3]))));
         };
-        const int left = w.tv - t0;
         if (left >= Q) {
 #pragma unroll
             for (int i = 0; i < Q; i += 4) {
@@ -235,14 +302,9 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = step(i + r);
                 if (MODE == 1) continue;
-                if constexpr (S >= 4) {              // part r of a channel keeps the sum of step i + r
-                    const float v = s == 0 ? y[0] : s == 1 ? y[1] : s == 2 ? y[2] : y[3];
-                    if (S == 4 || s < 4) s_y[MODE == 0 ? wv : 0][i + s % 4][c] = v;
-                } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (s == r % S) s_y[MODE == 0 ? wv : 0][i + r][c] = y[r];
-                }
+                for (int r = 0; r < 4; ++r) y[r] = pin(y[r]);
+                write_four<S>(s, [&](int which, auto pick) { s_y[MODE == 0 ? wv : 0][i + which][c] = pick(y); });
             }
         } else {                                     // the sequence ends inside this block
             for (int i = 0; i < left; ++i) {
@@ -252,14 +314,13 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
         }
         if (MODE == 0) {
             wave_sync();
-            X *yp = static_cast<X *>(a.y) + w.b * a.y_stride[0] + ed;
 #pragma unroll
             for (int j = 0; j < E; ++j) {
-                const int et = (lane + 64 * j) / CH;
-                if (!e_on || t0 + et >= w.tv) continue;
+                const int et = lane / CH + j * S;
+                if (!e_on || et >= left) continue;
                 float y = __builtin_fmaf(skip, u[j], s_y[MODE == 0 ? wv : 0][et][ec]);
                 if (a.z) y *= z[j] * sigmoid(z[j]);
-                yp[(long)(t0 + et) * a.y_stride[1]] = from_float<X>(y);
+                py.store(t0, j, y);
             }
         }
     }
@@ -335,7 +396,7 @@ __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const flo
 // sequence and one chunk: their sums over channels are joined in LDS and one row per workgroup goes to memory.
 // MODE 1 leaves the chunk's gradient at its start from a zero end and its sum of dt.
 template <typename X, int S, int MODE>
-__global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt, float *map_part,
+__global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt, float *map_part,
                                                               float *par_part) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
     __shared__ float4 s_step[kWaves][Q][CH];         // dt, dt * u, dy; then the step's sums g . b, A . w, c . h
@@ -355,11 +416,10 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a,
     if (!wave_on) w.nch = 0;
     set_time(w, pl, a.T, a.lengths);
     if (MODE == 1 && !wave_on) return;
-    Wave from = w;                                   // where a spare wave loads from (nothing is used)
-    if (!wave_on) from.nch = 1;
+    const int load_ch = wave_on ? w.nch : 1;         // a spare wave loads one channel and uses nothing of it
     const int c = lane / S, s = lane % S, ec = lane % CH;
     const bool e_on = ec < w.nch;
-    const int ed = w.d0 + min(ec, from.nch - 1);
+    const int ed = w.d0 + min(ec, load_ch - 1);
     const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f;
     const float skip = (MODE == 0 && a.skip) ? a.skip[ed] : 0.f;
     float a2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
@@ -376,17 +436,30 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a,
                 if (c < w.nch && 4 * s + k < a.N) g[k] = a.dfinal[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k];
         }
     }
-    Rows<X, S> ru, rd, rz, rg;
-    MapRows<X, S> rb, rc;
+    Rows<X, S> pu, pd, pz, pg, pdu, pdd, pdz;
+    Maps<X, S> pb, pc;
+    pd.init(a.delta, a.delta_stride, w.b, w.d0, load_ch);
+    pc.init(a.c, a.c_stride, w.b, w.g, a.N);
+    if (a.dy) pg.init(a.dy, a.dy_stride, w.b, w.d0, load_ch);
+    if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, load_ch);
+    if (MODE == 0) {
+        pu.init(a.u, a.u_stride, w.b, w.d0, load_ch);
+        pb.init(a.b, a.b_stride, w.b, w.g, a.N);
+        if (a.du) pdu.init(a.du, a.du_stride, w.b, w.d0, load_ch);
+        if (a.ddelta) pdd.init(a.ddelta, a.ddelta_stride, w.b, w.d0, load_ch);
+        if (a.dz) pdz.init(a.dz, a.dz_stride, w.b, w.d0, load_ch);
+    }
+    X ru[E], rd[E], rz[E], rg[E], rb[S], rc[S];
     float4 rh;
     auto request = [&](int t0) {
-        rd.load(a.delta, a.delta_stride, from, t0);
-        if (a.dy) rg.load(a.dy, a.dy_stride, from, t0);
-        rc.load(a.c, a.c_stride, from, a.N, t0);
-        if (a.z) rz.load(a.z, a.z_stride, from, t0);
+        const int left = w.tv - t0;
+        pd.load(rd, t0, left);
+        if (a.dy) pg.load(rg, t0, left);
+        pc.load(rc, t0, left);
+        if (a.z) pz.load(rz, t0, left);
         if (MODE == 0) {
-            ru.load(a.u, a.u_stride, from, t0);
-            rb.load(a.b, a.b_stride, from, a.N, t0);
+            pu.load(ru, t0, left);
+            pb.load(rb, t0, left);
             rh = reinterpret_cast<const float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)];
         }
     };
@@ -396,26 +469,26 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a,
     if (last >= w.t_lo) request(last);
     for (int t0 = last; t0 >= w.t_lo; t0 -= Q) {
         float u[E], z[E], out[E], dt[E], dy[E], slope[E];
+        const int left = w.tv - t0;                  // steps of this block that exist (Q or more: all)
         wave_sync();
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            const int et = (lane + 64 * j) / CH;
-            const bool on = e_on && t0 + et < w.tv;
-            u[j] = (MODE == 0 && on) ? to_float(ru.v[j]) : 0.f;
-            z[j] = a.z ? to_float(rz.v[j]) : 0.f;
-            out[j] = (a.dy && on) ? to_float(rg.v[j]) : 0.f;
-            const float raw = to_float(rd.v[j]) + bias;
+            const int et = lane / CH + j * S;
+            const bool on = e_on && et < left;
+            u[j] = (MODE == 0 && on) ? to_float(ru[j]) : 0.f;
+            z[j] = a.z ? to_float(rz[j]) : 0.f;
+            out[j] = (a.dy && on) ? to_float(rg[j]) : 0.f;
+            const float raw = to_float(rd[j]) + bias;
             dt[j] = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
             slope[j] = a.softplus ? sigmoid(raw) : 1.f;
             dy[j] = (a.z && on) ? out[j] * z[j] * sigmoid(z[j]) : out[j];
             s_step[wv][et][ec] = make_float4(dt[j], dt[j] * u[j], dy[j], 0.f);
         }
-        if (MODE == 0) rb.store(&s_b[wv][0][0], w, a.N, t0);
-        rc.store(&s_c[wv][0][0], w, a.N, t0);
+        if (MODE == 0) pb.to_lds(&s_b[wv][0][0], rb, a.N, left);
+        pc.to_lds(&s_c[wv][0][0], rc, a.N, left);
         const float h0[4] = {rh.x, rh.y, rh.z, rh.w};
         if (t0 > w.t_lo) request(t0 - Q);
         wave_sync();
-        const int left = w.tv - t0;                  // steps of this block that exist (Q or more: all)
         if (MODE == 1) {
             for (int i = min(left, Q) - 1; i >= 0; --i) {
                 const float4 v = s_step[wv][i][c];
@@ -442,37 +515,47 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a,
                     h[i][k] = __builtin_fmaf(decay[i][k], i ? h[i ? i - 1 : 0][k] : h0[k], v.y * bb[k]);
                 }
             }
+            // from the last step to the first, four at a time: their sums are written together
 #pragma unroll
-            for (int i = Q - 1; i >= 0; --i) {
-                if (!whole.value && i >= left) continue;
-                const float4 v = s_step[wv][i][c];
-                const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
-                const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
-                const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
-                float db[4], dc[4], gb = 0.f, aw = 0.f, ch = 0.f;
+            for (int i0 = Q - 4; i0 >= 0; i0 -= 4) {
+                float gb[4], aw[4], ch[4], sb[4], sc[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float gt = __builtin_fmaf(v.z, cc[k], g[k]);
-                    dc[k] = v.z * h[i][k];
-                    db[k] = v.y * gt;
-                    gb = __builtin_fmaf(gt, bb[k], gb);
-                    ch = __builtin_fmaf(cc[k], h[i][k], ch);
-                    g[k] = gt * decay[i][k];
-                    const float wk = g[k] * (i ? h[i ? i - 1 : 0][k] : h0[k]);
-                    aw = __builtin_fmaf(wk, a2[k], aw);
-                    blkA[k] = __builtin_fmaf(wk, v.x, blkA[k]);
+                for (int r = 3; r >= 0; --r) {
+                    const int i = i0 + r;
+                    gb[r] = aw[r] = ch[r] = sb[r] = sc[r] = 0.f;
+                    if (!whole.value && i >= left) continue;
+                    const float4 v = s_step[wv][i][c];
+                    const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
+                    const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
+                    const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
+                    float db[4], dc[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float gt = __builtin_fmaf(v.z, cc[k], g[k]);
+                        dc[k] = v.z * h[i][k];
+                        db[k] = v.y * gt;
+                        gb[r] = __builtin_fmaf(gt, bb[k], gb[r]);
+                        ch[r] = __builtin_fmaf(cc[k], h[i][k], ch[r]);
+                        g[k] = gt * decay[i][k];
+                        const float wk = g[k] * (i ? h[i ? i - 1 : 0][k] : h0[k]);
+                        aw[r] = __builtin_fmaf(wk, a2[k], aw[r]);
+                        blkA[k] = __builtin_fmaf(wk, v.x, blkA[k]);
+                    }
+                    gb[r] = pin(sum_parts<S>(gb[r]));
+                    aw[r] = pin(sum_parts<S>(aw[r]));
+                    ch[r] = pin(sum_parts<S>(ch[r]));
+                    sb[r] = pin(sum_channels<S>(db));
+                    sc[r] = pin(sum_channels<S>(dc));
                 }
-                gb = sum_parts<S>(gb);
-                aw = sum_parts<S>(aw);
-                if (a.z) ch = sum_parts<S>(ch);
-                const float sb = sum_channels<S>(db), sc = sum_channels<S>(dc);
-                if (s == 0) s_step[wv][i][c] = make_float4(gb, aw, ch, 0.f);
-                // lane (quarter q, part s) has the sums of state 4 s + value of quarter q
-                if (lane % 16 < S) {
-                    const int n = 4 * s + 2 * ((lane >> 4) & 1) + (lane >> 5);
-                    s_b[wv][i][n] = sb;
-                    s_c[wv][i][n] = sc;
-                }
+                write_four<S>(s, [&](int which, auto pick) {
+                    s_step[wv][i0 + which][c] = make_float4(pick(gb), pick(aw), pick(ch), 0.f);
+                });
+                // quarter q of the wave has, in part s of each of its channels, the sums of state 4 s + value of q
+                const int n = 4 * s + 2 * ((lane >> 4) & 1) + (lane >> 5);
+                write_four<16 / S>(lane % 16 / S, [&](int which, auto pick) {
+                    s_b[wv][i0 + which][n] = pick(sb);
+                    s_c[wv][i0 + which][n] = pick(sc);
+                });
             }
         };
         if (left >= Q) block(std::true_type{});
@@ -483,20 +566,19 @@ __global__ __launch_bounds__(64 * kWaves) void scan_bwd_kernel(tgru_scan_args a,
         float bs = 0.f, bb = 0.f;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-            const int et = (lane + 64 * j) / CH;
-            if (!e_on || t0 + et >= w.tv) continue;
+            const int et = lane / CH + j * S;
+            if (!e_on || et >= left) continue;
             const float4 r = s_step[wv][et][ec];
-            const long t = t0 + et;
             const float du = __builtin_fmaf(r.x, dt[j], skip * dy[j]);
             const float dd = __builtin_fmaf(r.x, u[j], kLn2 * r.y) * slope[j];
             bs = __builtin_fmaf(dy[j], u[j], bs);
             bb += dd;
-            if (a.du) static_cast<X *>(a.du)[w.b * a.du_stride[0] + t * a.du_stride[1] + ed] = from_float<X>(du);
-            if (a.ddelta) static_cast<X *>(a.ddelta)[w.b * a.ddelta_stride[0] + t * a.ddelta_stride[1] + ed] = from_float<X>(dd);
+            if (a.du) pdu.store(t0, j, du);
+            if (a.ddelta) pdd.store(t0, j, dd);
             if (a.dz) {
                 const float sg = sigmoid(z[j]);
                 const float v = out[j] * __builtin_fmaf(skip, u[j], r.z) * sg * __builtin_fmaf(z[j], 1.f - sg, 1.f);
-                static_cast<X *>(a.dz)[w.b * a.dz_stride[0] + t * a.dz_stride[1] + ed] = from_float<X>(v);
+                pdz.store(t0, j, v);
             }
         }
         dskip += bs;
@@ -768,6 +850,11 @@ int scan_call(const tgru_scan_args *a, bool backward, hipStream_t s) {
     const Plan pl = make_plan(a->B, a->T, a->D, a->N, a->G);
     if (backward ? !a->reserve || (a->dz && !a->z) : !a->y) return TGRU_E_NULL;
     if ((backward || pl.nchunks > 1) && !a->workspace) return TGRU_E_NULL;
+    auto wide = [](const void *p, const int64_t *stride) { return p && (stride[1] < 0 || stride[1] >= kMaxRowStride); };
+    if (wide(a->u, a->u_stride) || wide(a->delta, a->delta_stride) || wide(a->z, a->z_stride) || wide(a->b, a->b_stride) ||
+        wide(a->c, a->c_stride) || wide(a->y, a->y_stride) || wide(a->dy, a->dy_stride) || wide(a->du, a->du_stride) ||
+        wide(a->ddelta, a->ddelta_stride) || wide(a->dz, a->dz_stride))
+        return TGRU_E_DIMS;
     if (((uintptr_t)a->reserve & 15) || ((uintptr_t)a->workspace & 15)) return TGRU_E_ALIGN;
     if (int rc = check_device()) return rc;
     if (a->dtype == TGRU_DTYPE_F32) return run_scan_lanes<float>(*a, pl, backward, s);
