@@ -31,6 +31,7 @@ namespace tgru {
 namespace ssm {
 
 constexpr int Q = 16;                // steps per block
+constexpr int R = Q / 2;             // steps whose states the backward pass keeps in registers at a time
 constexpr int kWaves = 4;            // per workgroup
 constexpr int64_t kMaxRowStride = TGRU_SCAN_MAX_ROW_STRIDE;
 
@@ -54,6 +55,10 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
 }
+
+// A barrier of the workgroup for what it exchanges through LDS.  Unlike __syncthreads() it does not wait for the wave's
+// loads and stores in flight (the next block's rows, this block's gradients).
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
@@ -176,11 +181,21 @@ struct Maps {
     }
     __device__ __forceinline__ static void to_lds(float *lds, const X (&v)[S], int N, int left) {
         const int lane = threadIdx.x & 63;
+        if (left >= Q && N == NP) {
+#pragma unroll
+            for (int j = 0; j < S; ++j) lds[lane + 64 * j] = to_float(v[j]);
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < S; ++j)
             lds[lane + 64 * j] = (lane / NP + j * RPJ < left && lane % NP < N) ? to_float(v[j]) : 0.f;
     }
 };
+
+// What a step reads from LDS, fetched one step ahead: a read takes as long as two steps' arithmetic of the four states,
+// and the compiler, left alone, waits for each right behind it.  ahead() keeps the fetches in front of what follows.
+struct StepIn { float4 v, b, c; };
+__device__ __forceinline__ void ahead() { __builtin_amdgcn_sched_barrier(0); }
 
 // x, kept where it is: the compiler may not move the computation of x into a branch behind this point.
 __device__ __forceinline__ float pin(float x) {
@@ -268,39 +283,56 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
         float u[E], z[E];
         const int left = w.tv - t0;
         wave_sync();
+        // (a block that is there in full, in a wave whose channels all exist, needs no selection)
+        auto stage = [&](auto full) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const int et = lane / CH + j * S;
-            const bool on = e_on && et < left;
-            u[j] = on ? to_float(ru[j]) : 0.f;
-            z[j] = (MODE == 0 && a.z) ? to_float(rz[j]) : 0.f;
-            const float raw = to_float(rd[j]) + bias;
-            const float dt = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
-            s_step[wv][et][ec] = make_float2(dt, dt * u[j]);
-        }
+            for (int j = 0; j < E; ++j) {
+                const int et = lane / CH + j * S;
+                const bool on = full.value || (e_on && et < left);
+                u[j] = on ? to_float(ru[j]) : 0.f;
+                z[j] = (MODE == 0 && a.z) ? to_float(rz[j]) : 0.f;
+                const float raw = to_float(rd[j]) + bias;
+                const float dt = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
+                s_step[wv][et][ec] = make_float2(dt, dt * u[j]);
+            }
+        };
+        const bool full = left >= Q && w.nch == CH;
+        if (full) stage(std::true_type{});
+        else stage(std::false_type{});
         pb.to_lds(&s_b[wv][0][0], rb, a.N, left);
         if (MODE == 0) pc.to_lds(&s_c[wv][0][0], rc, a.N, left);
         if (left > Q) request(t0 + Q);
         wave_sync();
         if (MODE == 0 && a.reserve)
             reinterpret_cast<float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)] = make_float4(h[0], h[1], h[2], h[3]);
-        auto step = [&](int i) {
+        auto fetch = [&](int i) {
+            StepIn in;
             const float2 v = s_step[wv][i][c];
-            const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
-            const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+            in.v = make_float4(v.x, v.y, 0.f, 0.f);
+            in.b = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
+            if (MODE == 0) in.c = *reinterpret_cast<const float4 *>(&s_c[MODE == 0 ? wv : 0][i][4 * s]);
+            return in;
+        };
+        auto step = [&](const StepIn &in) {
+            const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(v.x * a2[k]), h[k], v.y * bb[k]);
-            if (MODE == 1) { dts += v.x; return 0.f; }
-            const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[MODE == 0 ? wv : 0][i][4 * s]);
-            return sum_parts<S>(__builtin_fmaf(c4.x, h[0], __builtin_fmaf(c4.y, h[1], __builtin_fmaf(c4.z, h[2], c4.w * h[3]))));
+                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(in.v.x * a2[k]), h[k], in.v.y * bb[k]);
+            if (MODE == 1) { dts += in.v.x; return 0.f; }
+            return sum_parts<S>(__builtin_fmaf(in.c.x, h[0], __builtin_fmaf(in.c.y, h[1], __builtin_fmaf(in.c.z, h[2], in.c.w * h[3]))));
         };
         if (left >= Q) {
+            StepIn next = fetch(0);
 #pragma unroll
             for (int i = 0; i < Q; i += 4) {
                 float y[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = step(i + r);
+                for (int r = 0; r < 4; ++r) {
+                    const StepIn in = next;
+                    if (i + r + 1 < Q) next = fetch(i + r + 1);
+                    ahead();
+                    y[r] = step(in);
+                }
                 if (MODE == 1) continue;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = pin(y[r]);
@@ -308,20 +340,24 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
             }
         } else {                                     // the sequence ends inside this block
             for (int i = 0; i < left; ++i) {
-                const float y = step(i);
+                const float y = step(fetch(i));
                 if (MODE == 0 && s == 0) s_y[MODE == 0 ? wv : 0][i][c] = y;
             }
         }
         if (MODE == 0) {
             wave_sync();
+            auto finish = [&](auto full) {
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const int et = lane / CH + j * S;
-                if (!e_on || et >= left) continue;
-                float y = __builtin_fmaf(skip, u[j], s_y[MODE == 0 ? wv : 0][et][ec]);
-                if (a.z) y *= z[j] * sigmoid(z[j]);
-                py.store(t0, j, y);
-            }
+                for (int j = 0; j < E; ++j) {
+                    const int et = lane / CH + j * S;
+                    if (!full.value && (!e_on || et >= left)) continue;
+                    float y = __builtin_fmaf(skip, u[j], s_y[MODE == 0 ? wv : 0][et][ec]);
+                    if (a.z) y *= z[j] * sigmoid(z[j]);
+                    py.store(t0, j, y);
+                }
+            };
+            if (full) finish(std::true_type{});
+            else finish(std::false_type{});
         }
     }
     if (MODE == 1) {
@@ -400,7 +436,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
                                                               float *par_part) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
     __shared__ float4 s_step[kWaves][Q][CH];         // dt, dt * u, dy; then the step's sums g . b, A . w, c . h
-    __shared__ __align__(16) float s_b[kWaves][Q][NP], s_c[kWaves][Q][NP];     // b and c; then the wave's db and dc
+    // b and c; then the wave's db and dc, which the workgroup joins while the next block fills the other buffer
+    constexpr int NB = MODE == 0 ? 2 : 1;
+    __shared__ __align__(16) float s_b2[NB][kWaves][Q][NP], s_c2[NB][kWaves][Q][NP];
+    int buf = 0;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Wave w;
     int id = blockIdx.x;
@@ -468,22 +507,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
     const int last = w.tv > w.t_lo ? w.t_lo + (w.tv - 1 - w.t_lo) / Q * Q : w.t_lo - Q;
     if (last >= w.t_lo) request(last);
     for (int t0 = last; t0 >= w.t_lo; t0 -= Q) {
-        float u[E], z[E], out[E], dt[E], dy[E], slope[E];
+        float u[E], z[E], out[E], dt[E], dy[E], slope[E], gate[E];
         const int left = w.tv - t0;                  // steps of this block that exist (Q or more: all)
+        auto &s_b = s_b2[buf], &s_c = s_c2[buf];
         wave_sync();
+        const bool full = left >= Q && w.nch == CH;
+        auto stage = [&](auto full) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const int et = lane / CH + j * S;
-            const bool on = e_on && et < left;
-            u[j] = (MODE == 0 && on) ? to_float(ru[j]) : 0.f;
-            z[j] = a.z ? to_float(rz[j]) : 0.f;
-            out[j] = (a.dy && on) ? to_float(rg[j]) : 0.f;
-            const float raw = to_float(rd[j]) + bias;
-            dt[j] = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
-            slope[j] = a.softplus ? sigmoid(raw) : 1.f;
-            dy[j] = (a.z && on) ? out[j] * z[j] * sigmoid(z[j]) : out[j];
-            s_step[wv][et][ec] = make_float4(dt[j], dt[j] * u[j], dy[j], 0.f);
-        }
+            for (int j = 0; j < E; ++j) {
+                const int et = lane / CH + j * S;
+                const bool on = full.value || (e_on && et < left);
+                u[j] = (MODE == 0 && on) ? to_float(ru[j]) : 0.f;
+                z[j] = a.z ? to_float(rz[j]) : 0.f;
+                out[j] = (a.dy && on) ? to_float(rg[j]) : 0.f;
+                const float raw = to_float(rd[j]) + bias;
+                dt[j] = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
+                slope[j] = a.softplus ? sigmoid(raw) : 1.f;
+                gate[j] = a.z ? sigmoid(z[j]) : 1.f;
+                dy[j] = (a.z && on) ? out[j] * z[j] * gate[j] : out[j];
+                s_step[wv][et][ec] = make_float4(dt[j], dt[j] * u[j], dy[j], 0.f);
+            }
+        };
+        if (full) stage(std::true_type{});
+        else stage(std::false_type{});
         if (MODE == 0) pb.to_lds(&s_b[wv][0][0], rb, a.N, left);
         pc.to_lds(&s_c[wv][0][0], rc, a.N, left);
         const float h0[4] = {rh.x, rh.y, rh.z, rh.w};
@@ -501,33 +547,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
             continue;
         }
         float blkA[4] = {0.f, 0.f, 0.f, 0.f};
-        auto block = [&](auto whole) {
-            float decay[Q][4], h[Q][4];
+        auto fetch = [&](int i, bool reverse) {
+            StepIn in;
+            in.v = s_step[wv][i][c];
+            in.b = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
+            if (reverse) in.c = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
+            return in;
+        };
+        auto advance = [&](const StepIn &in, const float (&from)[4], float (&to)[4], float (&decay)[4]) {
+            const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w};
 #pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                if (!whole.value && i >= left) continue;
-                const float4 v = s_step[wv][i][c];
-                const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
-                const float bb[4] = {b4.x, b4.y, b4.z, b4.w};
+            for (int k = 0; k < 4; ++k) {
+                decay[k] = __builtin_amdgcn_exp2f(in.v.x * a2[k]);
+                to[k] = __builtin_fmaf(decay[k], from[k], in.v.y * bb[k]);
+            }
+        };
+        // steps first .. first + R - 1 of the block, from state h0 in front of them; `next` is step `first`
+        auto part = [&](auto whole, auto first_, const float (&h0)[4], StepIn next) {
+            constexpr int first = first_.value;
+            float decay[R][4], h[R][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    decay[i][k] = __builtin_amdgcn_exp2f(v.x * a2[k]);
-                    h[i][k] = __builtin_fmaf(decay[i][k], i ? h[i ? i - 1 : 0][k] : h0[k], v.y * bb[k]);
-                }
+            for (int i = 0; i < R; ++i) {
+                const StepIn in = next;
+                next = i + 1 < R ? fetch(first + i + 1, false) : fetch(first + R - 1, true);
+                ahead();
+                if (!whole.value && first + i >= left) continue;
+                advance(in, i ? h[i ? i - 1 : 0] : h0, h[i], decay[i]);
             }
             // from the last step to the first, four at a time: their sums are written together
 #pragma unroll
-            for (int i0 = Q - 4; i0 >= 0; i0 -= 4) {
+            for (int i0 = R - 4; i0 >= 0; i0 -= 4) {
                 float gb[4], aw[4], ch[4], sb[4], sc[4];
 #pragma unroll
                 for (int r = 3; r >= 0; --r) {
                     const int i = i0 + r;
                     gb[r] = aw[r] = ch[r] = sb[r] = sc[r] = 0.f;
-                    if (!whole.value && i >= left) continue;
-                    const float4 v = s_step[wv][i][c];
-                    const float4 b4 = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
-                    const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
-                    const float bb[4] = {b4.x, b4.y, b4.z, b4.w}, cc[4] = {c4.x, c4.y, c4.z, c4.w};
+                    const StepIn in = next;
+                    if (i > 0) next = fetch(first + i - 1, true);
+                    ahead();
+                    if (!whole.value && first + i >= left) continue;
+                    const float4 v = in.v;
+                    const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cc[4] = {in.c.x, in.c.y, in.c.z, in.c.w};
                     float db[4], dc[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -548,15 +608,32 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
                     sc[r] = pin(sum_channels<S>(dc));
                 }
                 write_four<S>(s, [&](int which, auto pick) {
-                    s_step[wv][i0 + which][c] = make_float4(pick(gb), pick(aw), pick(ch), 0.f);
+                    s_step[wv][first + i0 + which][c] = make_float4(pick(gb), pick(aw), pick(ch), 0.f);
                 });
                 // quarter q of the wave has, in part s of each of its channels, the sums of state 4 s + value of q
                 const int n = 4 * s + 2 * ((lane >> 4) & 1) + (lane >> 5);
                 write_four<16 / S>(lane % 16 / S, [&](int which, auto pick) {
-                    s_b[wv][i0 + which][n] = pick(sb);
-                    s_c[wv][i0 + which][n] = pick(sc);
+                    s_b[wv][first + i0 + which][n] = pick(sb);
+                    s_c[wv][first + i0 + which][n] = pick(sc);
                 });
             }
+        };
+        // The states of R steps are kept in registers: the second half of the block first, from a state that is carried
+        // through the first half and forgotten again.
+        auto block = [&](auto whole) {
+            if (whole.value || left > R) {
+                float hm[4] = {h0[0], h0[1], h0[2], h0[3]}, decay[4];
+                StepIn next = fetch(0, false);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const StepIn in = next;
+                    next = fetch(i + 1, false);
+                    ahead();
+                    advance(in, hm, hm, decay);
+                }
+                part(whole, std::integral_constant<int, R>{}, hm, next);
+            }
+            part(whole, std::integral_constant<int, 0>{}, h0, fetch(0, false));
         };
         if (left >= Q) block(std::true_type{});
         else block(std::false_type{});
@@ -564,28 +641,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
         for (int k = 0; k < 4; ++k) dA[k] += blkA[k];
         wave_sync();
         float bs = 0.f, bb = 0.f;
+        auto finish = [&](auto full) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const int et = lane / CH + j * S;
-            if (!e_on || et >= left) continue;
-            const float4 r = s_step[wv][et][ec];
-            const float du = __builtin_fmaf(r.x, dt[j], skip * dy[j]);
-            const float dd = __builtin_fmaf(r.x, u[j], kLn2 * r.y) * slope[j];
-            bs = __builtin_fmaf(dy[j], u[j], bs);
-            bb += dd;
-            if (a.du) pdu.store(t0, j, du);
-            if (a.ddelta) pdd.store(t0, j, dd);
-            if (a.dz) {
-                const float sg = sigmoid(z[j]);
-                const float v = out[j] * __builtin_fmaf(skip, u[j], r.z) * sg * __builtin_fmaf(z[j], 1.f - sg, 1.f);
-                pdz.store(t0, j, v);
+            for (int j = 0; j < E; ++j) {
+                const int et = lane / CH + j * S;
+                if (!full.value && (!e_on || et >= left)) continue;
+                const float4 r = s_step[wv][et][ec];
+                const float du = __builtin_fmaf(r.x, dt[j], skip * dy[j]);
+                const float dd = __builtin_fmaf(r.x, u[j], kLn2 * r.y) * slope[j];
+                bs = __builtin_fmaf(dy[j], u[j], bs);
+                bb += dd;
+                if (a.du) pdu.store(t0, j, du);
+                if (a.ddelta) pdd.store(t0, j, dd);
+                if (a.dz)
+                    pdz.store(t0, j, out[j] * __builtin_fmaf(skip, u[j], r.z) * gate[j] * __builtin_fmaf(z[j], 1.f - gate[j], 1.f));
             }
-        }
+        };
+        if (full) finish(std::true_type{});
+        else finish(std::false_type{});
         dskip += bs;
         dbias += bb;
         if (map_part) {
             // the four waves' sums of this block, joined: map_part[b][g][workgroup][t][db, dc][NP]
-            __syncthreads();
+            lds_barrier();
             float *to = map_part + ((((long)w.b * a.G + w.g) * pl.wpg + wg) * a.T + t0) * 2 * NP;
             for (int e = threadIdx.x; e < 2 * Q * NP; e += 64 * kWaves) {
                 const int t = e / (2 * NP), n = e % (2 * NP);
@@ -595,7 +673,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
                 for (int q = 0; q < kWaves; ++q) v += n < NP ? s_b[q][t][n] : s_c[q][t][n - NP];
                 to[e] = v;
             }
-            __syncthreads();
+            buf ^= NB - 1;
         }
     }
     if (MODE == 1) {
