@@ -153,7 +153,7 @@ def test_size_queries(tg):
     lb = tg.lib()
     assert lb.tgru_scan_reserve_bytes(0, 1, 1, 1, 1) == 0 and lb.tgru_scan_workspace_bytes(1, 1, 1, 65, 1, 1) == 0
     assert lb.tgru_conv_backward_workspace_bytes(1, 1, 1, 9) == 0
-    # a state of 16 fp32 values in front of every 16 steps: one fp32 value per step and channel (channels in waves of 16)
+    # 16 fp32 states in front of every 16 steps: one fp32 value per step and channel
     assert lb.tgru_scan_reserve_bytes(2, 64, 48, 16, 1) == 2 * 64 * 48 * 4
     assert lb.tgru_scan_workspace_bytes(64, 256, 1024, 16, 1, 0) == 0         # enough channels: time is not cut
     assert lb.tgru_scan_workspace_bytes(1, 4096, 64, 16, 1, 0) > 0

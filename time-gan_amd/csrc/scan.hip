@@ -5,25 +5,29 @@
 // What bounds it.  A step costs, per channel AND STATE, one exponential and four multiply-adds forward, and about
 // eighteen operations and the exponential backward, against a few bytes per channel: with 16 states the vector ALU and
 // not HBM is the limit.  The matrix instructions do not apply: every (channel, state) pair has a decay of its own at
-// every step, so no product of two matrices is shared by two steps.  Hence:
-//   * the exponentials are computed once per pass and kept in registers where the backward pass needs them again;
-//   * everything that is per channel only (softplus, dt u, the gate) is computed once per (step, channel), by lanes that
-//     split a block of 16 steps among themselves, and handed to the recurrence through LDS;
-//   * sums over the states of a channel and over the channels of a group are joined inside the wave with DPP adds and
-//     permlane swaps.
+// every step, so no product of two matrices is shared by two steps.  What the vector ALU of this chip does in how many
+// cycles per wave (measured, two or more waves per SIMD): 4-byte multiplies, adds and multiply-adds 2.5, 8-byte ones,
+// DPP adds, selects and conversions 4.3, exp2 / log2 / reciprocal 8.2, permlane swaps 8.3; with one wave, 5 at least.
+// So: enough waves, operands that fit the short encodings, few selects, and no instruction for what is the same in a
+// whole wave.
 //
-// Layout.  A wave owns CH = 64 / S channels: S lanes per channel, four states each (S = 1, 2, 4, 8, 16 covers 64 states;
-// states beyond N are zeros throughout).  Lane = channel * S + part.  A block of Q = 16 steps is staged in LDS (dt, dt u,
-// b, c in fp32), the next block's rows are requested before the recurrence runs over this one.  Nothing is shared between
-// waves in the forward pass: there is no barrier.
+// Layout.  A wave owns CH = 64 / S channels of one group: S lanes per channel, four states each (S = 2, 4, 8, 16 covers
+// 64 states; states beyond N are zeros throughout), lane = channel * S + part.  A block of Q = 16 steps is staged in LDS:
+// what is per channel only (softplus, dt u, the gate) is computed once per (step, channel) by lanes that split the block
+// among themselves, the maps' rows are brought to fp32; the next block's rows are requested before the recurrence runs
+// over this one.  (Tried instead: a lane with all 16 states of a channel and the maps through the scalar cache -- an eighth
+// fewer instructions, but a quarter of the waves: 139 us against 91 on a batch of 64 windows of 256 steps with 1024
+// channels, equal on one sequence of 16384.)
 //
-// Time is split into chunks when there are too few channels to fill the chip (chunk_plan): a first pass leaves each
+// scan_bwd_kernel needs the states of every step in reverse.  The forward pass saves the state in front of every block
+// (4 bytes per step, channel and 16 states); inside a block the states are computed again, R steps in registers at a time.
+// Sums over the states of a channel and over the channels of a group are joined inside the wave with DPP adds and permlane
+// swaps.
+//
+// Time is split into chunks when there are too few channels to fill the chip (make_plan): a first pass leaves each
 // chunk's end state from a zero start and its sum of dt -- the chunk multiplies an incoming state by exp(A sum dt) --, a
 // second kernel joins the chunks in order, and the main pass starts every chunk from its joined state.  The backward
 // pass does the same from the other end.
-//
-// For the backward pass the forward pass saves the state in front of every block of 16 steps (4 bytes per step, channel
-// and 16 states); the states inside a block are computed again from it, 16 steps in registers at a time.
 #include "ssm_common.h"
 #include <type_traits>
 
@@ -35,19 +39,19 @@ constexpr int R = Q / 2;             // steps whose states the backward pass kee
 constexpr int kWaves = 4;            // per workgroup
 constexpr int64_t kMaxRowStride = TGRU_SCAN_MAX_ROW_STRIDE;
 
-struct Plan {                        // how a call is cut up; made on the host
-    int S, CH;                       // lanes per channel, channels per wave
-    int Dg, tpg, tiles;              // channels per group, waves per group, waves per sequence and chunk
-    int wpg;                         // backward: workgroups per group
+// make_plan's limits, in waves: enough of them without chunks, and what chunks are cut for.
+constexpr long kEnoughWaves = 768, kFullWaves = 4096;
+
+struct Plan {                        // how a pass is cut up; made on the host
+    int NP, CH, Dg;                  // states with padding (8 .. 64), channels per wave, channels per group
+    int tpg, tiles, wpg;             // waves per group, per sequence and chunk; workgroups per group (scan_bwd_kernel)
     int nblk;                        // blocks of Q steps
     int nchunks, chunk;              // chunks of time, steps of one (a multiple of Q)
+    int quads;                       // the maps' rows can be loaded four values at a time
 };
 
-// What goes between kernels, per wave-lane: float4 carry[b][chunk][tile][64], float sdt[b][chunk][tile][64],
-// float4 ckpt[b][block][tile][64].
-__device__ __forceinline__ long lane_slot(const Plan &pl, int b, int outer, int nouter, int tile) {
-    return (((long)b * nouter + outer) * pl.tiles + tile) * 64 + (threadIdx.x & 63);
-}
+// What goes between kernels, all fp32: ckpt [b][block][d][NP] (the state in front of each block), carry [b][chunk][d][NP],
+// sdt [b][chunk][d].
 
 // LDS written by some lanes of a wave and read by others: the LDS unit takes a wave's accesses in order, so all that
 // has to be held back is the compiler.
@@ -95,26 +99,12 @@ __device__ __forceinline__ float sum_channels(const float (&v)[4]) {
 }
 
 // A wave's place: channels [d0, d0 + nch) of group g of sequence b, steps [t_lo, t_hi) of which [t_lo, tv) exist.
-struct Wave { int b, chunk, tile, g, d0, nch, t_lo, t_hi, tv; };
+struct Wave { int b, chunk, g, d0, nch, t_lo, t_hi, tv; };
 
-__device__ __forceinline__ void set_tile(Wave &w, const Plan &pl, int tile_in_group) {
-    w.tile = w.g * pl.tpg + tile_in_group;
-    w.d0 = w.g * pl.Dg + tile_in_group * pl.CH;
-    w.nch = min(pl.CH, pl.Dg - tile_in_group * pl.CH);
-}
 __device__ __forceinline__ void set_time(Wave &w, const Plan &pl, int T, const int32_t *lengths) {
     w.t_lo = w.chunk * pl.chunk;
     w.t_hi = min(T, w.t_lo + pl.chunk);
     w.tv = min(w.t_hi, clamped_length(lengths, w.b, T));
-}
-
-// The decays' exponents per unit of dt, to base 2, of this lane's four states (0 for states that do not exist).
-__device__ __forceinline__ void load_rates(const float *a, int N, const Wave &w, int c, int s, float (&a2)[4]) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int n = 4 * s + k;
-        a2[k] = (c < w.nch && n < N) ? a[(long)(w.d0 + c) * N + n] * kLog2e : 0.f;
-    }
 }
 
 // Rows of a tensor of one block, split over the lanes.  All addresses are a base that is the same for the whole wave (and
@@ -153,42 +143,50 @@ struct Rows {
     }
 };
 
-// b or c: NP = 4 S values a step (zeros beyond N and behind the end), element j of a lane is value lane % NP of step
-// lane / NP + j 64 / NP.
+// Rows of b or c of a block on their way to LDS, in fp32, zeros beyond N and behind the end: Q rows of S quads of values,
+// a quad per lane and element.
 template <typename X, int S>
 struct Maps {
-    static constexpr int NP = 4 * S, RPJ = 64 / NP;
+    static constexpr int F = Q * S, V = F < 64 ? 1 : F / 64;           // quads in all, per lane
+    struct alignas(4 * sizeof(X)) Quad { X v[4]; };
     const char *base;
     long row;
-    unsigned lane_off, col;
-    __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int g, int N) {
-        const int lane = threadIdx.x & 63;
+    Quad q[V];
+    __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int g) {
         base = reinterpret_cast<const char *>(static_cast<const X *>(p) + b * stride[0] + g * stride[2]);
         row = stride[1] * (long)sizeof(X);
-        col = min(lane % NP, N - 1) * (unsigned)sizeof(X);
-        lane_off = (unsigned)(lane / NP) * (unsigned)row + col;
     }
-    __device__ __forceinline__ void load(X (&v)[S], int t0, int left) const {
-        const char *p = base + t0 * row;
-        if (left >= Q) {
-#pragma unroll
-            for (int j = 0; j < S; ++j, p += RPJ * row) v[j] = *reinterpret_cast<const X *>(p + lane_off);
-        } else {
-#pragma unroll
-            for (int j = 0; j < S; ++j)
-                v[j] = *reinterpret_cast<const X *>(p + ((unsigned)min((int)(threadIdx.x & 63) / NP + j * RPJ, left - 1) * (unsigned)row + col));
-        }
-    }
-    __device__ __forceinline__ static void to_lds(float *lds, const X (&v)[S], int N, int left) {
+    // quads: every row starts on a quad and N is a multiple of 4 -- one load instead of four
+    __device__ __forceinline__ void load(int t0, int left, int N, int quads) {
         const int lane = threadIdx.x & 63;
-        if (left >= Q && N == NP) {
+        const char *p = base + t0 * row;
+        const int first = lane / S, rows = min(left, Q) - 1;
 #pragma unroll
-            for (int j = 0; j < S; ++j) lds[lane + 64 * j] = to_float(v[j]);
-            return;
+        for (int j = 0; j < V; ++j) {
+            const char *r = p + (unsigned)min(first + j * (64 / S), rows) * (unsigned)row;
+            if (quads) {
+                q[j] = *reinterpret_cast<const Quad *>(r + min(4 * (lane % S), N - 4) * (unsigned)sizeof(X));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[j].v[k] = *reinterpret_cast<const X *>(r + min(4 * (lane % S) + k, N - 1) * (unsigned)sizeof(X));
+            }
         }
+    }
+    __device__ __forceinline__ void to_lds(float *lds, int left, int N) const {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-        for (int j = 0; j < S; ++j)
-            lds[lane + 64 * j] = (lane / NP + j * RPJ < left && lane % NP < N) ? to_float(v[j]) : 0.f;
+        for (int j = 0; j < V; ++j) {
+            const int t = lane / S + j * (64 / S), n = 4 * (lane % S);
+            float4 f;
+            f.x = to_float(q[j].v[0]); f.y = to_float(q[j].v[1]); f.z = to_float(q[j].v[2]); f.w = to_float(q[j].v[3]);
+            if (left < Q || N < 4 * S) {
+                f.x = (t < left && n < N) ? f.x : 0.f;
+                f.y = (t < left && n + 1 < N) ? f.y : 0.f;
+                f.z = (t < left && n + 2 < N) ? f.z : 0.f;
+                f.w = (t < left && n + 3 < N) ? f.w : 0.f;
+            }
+            if (F >= 64 || lane < F) reinterpret_cast<float4 *>(lds)[lane + 64 * j] = f;
+        }
     }
 };
 
@@ -221,60 +219,94 @@ __device__ __forceinline__ void write_four(int replica, F &&write) {
     }
 }
 
+// A wave of the passes whose waves are independent of each other; false where there is none.
+__device__ __forceinline__ bool place_wave(Wave &w, const tgru_scan_args &a, const Plan &pl) {
+    const unsigned id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned rest = id / (unsigned)pl.tiles, flat = id - rest * (unsigned)pl.tiles;
+    w.b = (int)(rest / (unsigned)pl.nchunks);
+    if (w.b >= a.B) return false;
+    w.chunk = (int)(rest - (unsigned)w.b * (unsigned)pl.nchunks);
+    w.g = (int)(flat / (unsigned)pl.tpg);
+    const int in_group = (int)flat - w.g * pl.tpg;
+    w.d0 = w.g * pl.Dg + in_group * pl.CH;
+    w.nch = min(pl.CH, pl.Dg - in_group * pl.CH);
+    set_time(w, pl, a.T, a.lengths);
+    return true;
+}
+
+// This lane's four states: where they are in a row of carry or ckpt, and their rates to base 2 per unit of dt.
+template <int S>
+struct Lane {
+    int c, s;                        // channel of the wave, part of the channel
+    bool on;
+    long at;
+    float a2[4];
+    __device__ __forceinline__ void init(const float *rates, int N, const Wave &w) {
+        c = (threadIdx.x & 63) / S;
+        s = (threadIdx.x & 63) % S;
+        on = c < w.nch;
+        at = (long)(w.d0 + (on ? c : 0)) * (4 * S) + 4 * s;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a2[k] = has(k, N) ? rates[(long)(w.d0 + c) * N + 4 * s + k] * kLog2e : 0.f;
+    }
+    __device__ __forceinline__ bool has(int k, int N) const { return on && 4 * s + k < N; }
+    // from / to a (B, D, N) tensor
+    __device__ __forceinline__ void load(const float *t, const Wave &w, int D, int N, float (&v)[4]) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = has(k, N) ? t[((long)w.b * D + w.d0 + c) * N + 4 * s + k] : 0.f;
+    }
+    __device__ __forceinline__ void store(float *t, const Wave &w, int D, int N, const float (&v)[4]) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (has(k, N)) t[((long)w.b * D + w.d0 + c) * N + 4 * s + k] = v[k];
+    }
+};
+
+__device__ __forceinline__ void unpack(const float4 &f, float (&v)[4]) { v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
+
 // MODE 0: the outputs.  MODE 1: a chunk's end state from a zero start and its sum of dt, for the joining kernel.
 template <typename X, int S, int MODE>
 __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
-    constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
-    __shared__ float2 s_step[kWaves][Q][CH];                        // dt, dt * u
-    __shared__ __align__(16) float s_b[kWaves][Q][NP], s_c[MODE == 0 ? kWaves : 1][Q][NP];
-    __shared__ float s_y[MODE == 0 ? kWaves : 1][Q][CH];
+    constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64, M = MODE == 0 ? 2 : 1;
+    __shared__ float2 s_steps[kWaves][Q][CH];                           // dt, dt * u
+    __shared__ __align__(16) float s_maps[kWaves][M][Q][NP];            // b, c
+    __shared__ __align__(16) float s_ys[MODE == 0 ? kWaves : 1][Q][64]; // the lanes' shares of c . h
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long id = (long)blockIdx.x * kWaves + wv;
+    auto &s_step = s_steps[wv];
+    auto &s_map = s_maps[wv];
+    auto &s_y = s_ys[MODE == 0 ? wv : 0];
     Wave w;
-    const int flat = (int)(id % pl.tiles);
-    const long rest = id / pl.tiles;
-    w.chunk = (int)(rest % pl.nchunks);
-    if (rest / pl.nchunks >= a.B) return;
-    w.b = (int)(rest / pl.nchunks);
-    w.g = flat / pl.tpg;
-    set_tile(w, pl, flat - w.g * pl.tpg);
-    set_time(w, pl, a.T, a.lengths);
-    const int c = lane / S, s = lane % S;
-    const int ec = lane % CH;                                       // this lane's channel when it works per channel
+    if (!place_wave(w, a, pl)) return;
+    Lane<S> me;
+    me.init(a.a, a.N, w);
+    const int ec = lane % CH, ed = w.d0 + min(ec, w.nch - 1);           // this lane's channel when it works per channel
     const bool e_on = ec < w.nch;
-    const int ed = w.d0 + min(ec, w.nch - 1);
-    const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f;
-    const float skip = (MODE == 0 && a.skip) ? a.skip[ed] : 0.f;
-    float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
-    load_rates(a.a, a.N, w, c, s, a2);
+    const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f, skip = (MODE == 0 && a.skip) ? a.skip[ed] : 0.f;
+    float h[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
+    float4 *state = reinterpret_cast<float4 *>(carry + ((long)w.b * pl.nchunks + w.chunk) * a.D * NP + me.at);
     if (MODE == 0) {
-        if (pl.nchunks > 1) {
-            const float4 v = reinterpret_cast<const float4 *>(carry)[lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile)];
-            h[0] = v.x; h[1] = v.y; h[2] = v.z; h[3] = v.w;
-        } else if (a.initial_state) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (c < w.nch && 4 * s + k < a.N) h[k] = a.initial_state[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k];
-        }
+        if (pl.nchunks > 1) { if (me.on) unpack(*state, h); }
+        else if (a.initial_state) me.load(a.initial_state, w, a.D, a.N, h);
     }
+    float *ckpt = (MODE == 0 && a.reserve) ? a.reserve + (long)w.b * pl.nblk * a.D * NP + me.at : nullptr;
     Rows<X, S> pu, pd, pz, py;
-    Maps<X, S> pb, pc;
+    Maps<X, S> mb, mc;
     pu.init(a.u, a.u_stride, w.b, w.d0, w.nch);
     pd.init(a.delta, a.delta_stride, w.b, w.d0, w.nch);
-    pb.init(a.b, a.b_stride, w.b, w.g, a.N);
+    mb.init(a.b, a.b_stride, w.b, w.g);
     if (MODE == 0) {
         py.init(a.y, a.y_stride, w.b, w.d0, w.nch);
-        pc.init(a.c, a.c_stride, w.b, w.g, a.N);
+        mc.init(a.c, a.c_stride, w.b, w.g);
         if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, w.nch);
     }
-    X ru[E], rd[E], rz[E], rb[S], rc[S];
+    X ru[E], rd[E], rz[E];
     auto request = [&](int t0) {
         const int left = w.tv - t0;
         pu.load(ru, t0, left);
         pd.load(rd, t0, left);
-        pb.load(rb, t0, left);
+        mb.load(t0, left, a.N, pl.quads);
         if (MODE == 0) {
-            pc.load(rc, t0, left);
+            mc.load(t0, left, a.N, pl.quads);
             if (a.z) pz.load(rz, t0, left);
         }
     };
@@ -293,56 +325,45 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
                 z[j] = (MODE == 0 && a.z) ? to_float(rz[j]) : 0.f;
                 const float raw = to_float(rd[j]) + bias;
                 const float dt = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
-                s_step[wv][et][ec] = make_float2(dt, dt * u[j]);
+                s_step[et][ec] = make_float2(dt, dt * u[j]);
             }
         };
         const bool full = left >= Q && w.nch == CH;
         if (full) stage(std::true_type{});
         else stage(std::false_type{});
-        pb.to_lds(&s_b[wv][0][0], rb, a.N, left);
-        if (MODE == 0) pc.to_lds(&s_c[wv][0][0], rc, a.N, left);
+        mb.to_lds(&s_map[0][0][0], left, a.N);
+        if (MODE == 0) mc.to_lds(&s_map[M - 1][0][0], left, a.N);
         if (left > Q) request(t0 + Q);
         wave_sync();
-        if (MODE == 0 && a.reserve)
-            reinterpret_cast<float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)] = make_float4(h[0], h[1], h[2], h[3]);
+        if (ckpt && me.on) *reinterpret_cast<float4 *>(ckpt + (long)(t0 / Q) * a.D * NP) = make_float4(h[0], h[1], h[2], h[3]);
         auto fetch = [&](int i) {
             StepIn in;
-            const float2 v = s_step[wv][i][c];
+            const float2 v = s_step[i][me.c];
             in.v = make_float4(v.x, v.y, 0.f, 0.f);
-            in.b = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
-            if (MODE == 0) in.c = *reinterpret_cast<const float4 *>(&s_c[MODE == 0 ? wv : 0][i][4 * s]);
+            in.b = *reinterpret_cast<const float4 *>(&s_map[0][i][4 * me.s]);
+            if (MODE == 0) in.c = *reinterpret_cast<const float4 *>(&s_map[M - 1][i][4 * me.s]);
             return in;
         };
-        auto step = [&](const StepIn &in) {
-            const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w};
+        auto step = [&](int i, const StepIn &in) {
+            float bb[4];
+            unpack(in.b, bb);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(in.v.x * a2[k]), h[k], in.v.y * bb[k]);
-            if (MODE == 1) { dts += in.v.x; return 0.f; }
-            return sum_parts<S>(__builtin_fmaf(in.c.x, h[0], __builtin_fmaf(in.c.y, h[1], __builtin_fmaf(in.c.z, h[2], in.c.w * h[3]))));
+                h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(in.v.x * me.a2[k]), h[k], in.v.y * bb[k]);
+            if (MODE == 1) dts += in.v.x;
+            else s_y[i][lane] = __builtin_fmaf(in.c.x, h[0], __builtin_fmaf(in.c.y, h[1], __builtin_fmaf(in.c.z, h[2], in.c.w * h[3])));
         };
         if (left >= Q) {
             StepIn next = fetch(0);
 #pragma unroll
-            for (int i = 0; i < Q; i += 4) {
-                float y[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const StepIn in = next;
-                    if (i + r + 1 < Q) next = fetch(i + r + 1);
-                    ahead();
-                    y[r] = step(in);
-                }
-                if (MODE == 1) continue;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = pin(y[r]);
-                write_four<S>(s, [&](int which, auto pick) { s_y[MODE == 0 ? wv : 0][i + which][c] = pick(y); });
+            for (int i = 0; i < Q; ++i) {
+                const StepIn in = next;
+                if (i + 1 < Q) next = fetch(i + 1);
+                ahead();
+                step(i, in);
             }
         } else {                                     // the sequence ends inside this block
-            for (int i = 0; i < left; ++i) {
-                const float y = step(fetch(i));
-                if (MODE == 0 && s == 0) s_y[MODE == 0 ? wv : 0][i][c] = y;
-            }
+            for (int i = 0; i < left; ++i) step(i, fetch(i));
         }
         if (MODE == 0) {
             wave_sync();
@@ -351,7 +372,9 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
                 for (int j = 0; j < E; ++j) {
                     const int et = lane / CH + j * S;
                     if (!full.value && (!e_on || et >= left)) continue;
-                    float y = __builtin_fmaf(skip, u[j], s_y[MODE == 0 ? wv : 0][et][ec]);
+                    float y = skip * u[j];
+#pragma unroll
+                    for (int q = 0; q < S; ++q) y += s_y[et][ec * S + q];
                     if (a.z) y *= z[j] * sigmoid(z[j]);
                     py.store(t0, j, y);
                 }
@@ -361,65 +384,124 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
         }
     }
     if (MODE == 1) {
-        const long at = lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile);
-        reinterpret_cast<float4 *>(carry)[at] = make_float4(h[0], h[1], h[2], h[3]);
-        sdt[at] = dts;
+        if (!me.on) return;
+        *state = make_float4(h[0], h[1], h[2], h[3]);
+        if (me.s == 0) sdt[((long)w.b * pl.nchunks + w.chunk) * a.D + w.d0 + me.c] = dts;
         return;
     }
-    X *yp = static_cast<X *>(a.y) + w.b * a.y_stride[0] + ed;
     for (int t = max(w.t_lo, w.tv) + lane / CH; t < w.t_hi; t += S)
-        if (e_on) yp[(long)t * a.y_stride[1]] = from_float<X>(0.f);
-    if (a.final_state && w.chunk == pl.nchunks - 1 && c < w.nch) {
+        if (e_on) static_cast<X *>(a.y)[w.b * a.y_stride[0] + t * a.y_stride[1] + ed] = from_float<X>(0.f);
+    if (a.final_state && w.chunk == pl.nchunks - 1) me.store(a.final_state, w, a.D, a.N, h);
+}
+
+// The gradient that a chunk hands to the one before it, from zero behind its end, and its sum of dt.
+template <typename X, int S>
+__global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
+    constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
+    __shared__ float2 s_steps[kWaves][Q][CH];                           // dt, dy
+    __shared__ __align__(16) float s_maps[kWaves][Q][NP];               // c
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    auto &s_step = s_steps[wv];
+    auto &s_map = s_maps[wv];
+    Wave w;
+    if (!place_wave(w, a, pl)) return;
+    Lane<S> me;
+    me.init(a.a, a.N, w);
+    const int ec = lane % CH;
+    const bool e_on = ec < w.nch;
+    const float bias = a.delta_bias ? a.delta_bias[w.d0 + min(ec, w.nch - 1)] : 0.f;
+    float g[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
+    Rows<X, S> pd, pz, pg;
+    Maps<X, S> mc;
+    pd.init(a.delta, a.delta_stride, w.b, w.d0, w.nch);
+    mc.init(a.c, a.c_stride, w.b, w.g);
+    if (a.dy) pg.init(a.dy, a.dy_stride, w.b, w.d0, w.nch);
+    if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, w.nch);
+    X rd[E], rz[E], rg[E];
+    auto request = [&](int t0) {
+        const int left = w.tv - t0;
+        pd.load(rd, t0, left);
+        if (a.dy) pg.load(rg, t0, left);
+        if (a.z) pz.load(rz, t0, left);
+        mc.load(t0, left, a.N, pl.quads);
+    };
+    const int last = w.tv > w.t_lo ? w.t_lo + (w.tv - 1 - w.t_lo) / Q * Q : w.t_lo - Q;
+    if (last >= w.t_lo) request(last);
+    for (int t0 = last; t0 >= w.t_lo; t0 -= Q) {
+        const int left = w.tv - t0;
+        wave_sync();
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (4 * s + k < a.N) a.final_state[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k] = h[k];
+        for (int j = 0; j < E; ++j) {
+            const int et = lane / CH + j * S;
+            const bool on = e_on && et < left;
+            const float raw = to_float(rd[j]) + bias;
+            float dy = a.dy ? to_float(rg[j]) : 0.f;
+            if (a.z) { const float z = to_float(rz[j]); dy *= z * sigmoid(z); }
+            s_step[et][ec] = make_float2(on ? (a.softplus ? softplus(raw) : raw) : 0.f, on ? dy : 0.f);
+        }
+        mc.to_lds(&s_map[0][0], left, a.N);
+        if (t0 > w.t_lo) request(t0 - Q);
+        wave_sync();
+        auto fetch = [&](int i) {
+            StepIn in;
+            const float2 v = s_step[i][me.c];
+            in.v = make_float4(v.x, v.y, 0.f, 0.f);
+            in.c = *reinterpret_cast<const float4 *>(&s_map[i][4 * me.s]);
+            return in;
+        };
+        auto step = [&](const StepIn &in) {
+            float cc[4];
+            unpack(in.c, cc);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) g[k] = __builtin_amdgcn_exp2f(in.v.x * me.a2[k]) * __builtin_fmaf(in.v.y, cc[k], g[k]);
+            dts += in.v.x;
+        };
+        if (left >= Q) {
+            StepIn next = fetch(Q - 1);
+#pragma unroll
+            for (int i = Q - 1; i >= 0; --i) {
+                const StepIn in = next;
+                if (i > 0) next = fetch(i - 1);
+                ahead();
+                step(in);
+            }
+        } else {
+            for (int i = left - 1; i >= 0; --i) step(fetch(i));
+        }
     }
+    if (!me.on) return;
+    *reinterpret_cast<float4 *>(carry + ((long)w.b * pl.nchunks + w.chunk) * a.D * NP + me.at) = make_float4(g[0], g[1], g[2], g[3]);
+    if (me.s == 0) sdt[((long)w.b * pl.nchunks + w.chunk) * a.D + w.d0 + me.c] = dts;
 }
 
 // Joins the chunks: carry[chunk] becomes what enters the chunk.  `edge`: (B, D, N) entering the first chunk in the
-// order of the pass (the initial state forward, the final state's gradient backward), or null.
-template <int S>
-__global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const float *edge, Plan pl, int D, int N, int backward,
+// order of the pass (the initial state forward, the final state's gradient backward), or null.  One thread per state.
+__global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const float *edge, Plan pl, int B, int D, int N, int backward,
                                                        float *carry, const float *sdt) {
-    constexpr int CH = 64 / S;
-    const int lane = threadIdx.x, c = lane / S, s = lane % S;
-    Wave w;
-    w.b = blockIdx.x / pl.tiles;
-    const int flat = blockIdx.x - w.b * pl.tiles;
-    w.g = flat / pl.tpg;
-    set_tile(w, pl, flat - w.g * pl.tpg);
-    (void)CH;
-    float a2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
-    load_rates(a, N, w, c, s, a2);
-    if (edge && c < w.nch) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (4 * s + k < N) h[k] = edge[((long)w.b * D + w.d0 + c) * N + 4 * s + k];
-    }
+    const long id = (long)blockIdx.x * 64 + threadIdx.x, per = (long)D * pl.NP;
+    const int b = (int)(id / per);
+    if (b >= B) return;
+    const int e = (int)(id - b * per), d = e / pl.NP, n = e - d * pl.NP;
+    const float a2 = n < N ? a[(long)d * N + n] * kLog2e : 0.f;
+    float h = (edge && n < N) ? edge[((long)b * D + d) * N + n] : 0.f;
+    float *state = carry + (long)b * pl.nchunks * per + e;
+    const float *sums = sdt + (long)b * pl.nchunks * D + d;
     constexpr int U = 8;                 // chunks requested together
     for (int i0 = 0; i0 < pl.nchunks; i0 += U) {
-        float4 v[U];
-        float dt[U];
+        float v[U], dt[U];
 #pragma unroll
         for (int r = 0; r < U; ++r) {
-            const int i = min(i0 + r, pl.nchunks - 1);
-            const long at = lane_slot(pl, w.b, backward ? pl.nchunks - 1 - i : i, pl.nchunks, w.tile);
-            v[r] = reinterpret_cast<const float4 *>(carry)[at];
-            dt[r] = sdt[at];
+            const int i = min(i0 + r, pl.nchunks - 1), at = backward ? pl.nchunks - 1 - i : i;
+            v[r] = state[at * per];
+            dt[r] = sums[(long)at * D];
         }
 #pragma unroll
         for (int r = 0; r < U; ++r) {
             if (i0 + r >= pl.nchunks) break;
-            const int i = i0 + r;
-            const long at = lane_slot(pl, w.b, backward ? pl.nchunks - 1 - i : i, pl.nchunks, w.tile);
-            reinterpret_cast<float4 *>(carry)[at] = make_float4(h[0], h[1], h[2], h[3]);
-            const float e[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                // a chunk without steps passes the state on as it is, also where A is infinite
-                const float p = dt[r] == 0.f ? 1.f : __builtin_amdgcn_exp2f(dt[r] * a2[k]);
-                h[k] = __builtin_fmaf(p, h[k], e[k]);
-            }
+            state[(backward ? pl.nchunks - 1 - (i0 + r) : i0 + r) * per] = h;
+            // a chunk without steps passes the state on as it is, also where A is infinite
+            const float p = dt[r] == 0.f ? 1.f : __builtin_amdgcn_exp2f(dt[r] * a2);
+            h = __builtin_fmaf(p, h, v[r]);
         }
     }
 }
@@ -430,77 +512,65 @@ __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const flo
 //     d(dt_t) = u_t (g_t . b_t) + A . w_t          dA = sum over steps dt_t w_t
 // where dy is the gradient in front of the gate.  The four waves of a workgroup are neighbouring waves of one group, one
 // sequence and one chunk: their sums over channels are joined in LDS and one row per workgroup goes to memory.
-// MODE 1 leaves the chunk's gradient at its start from a zero end and its sum of dt.
-template <typename X, int S, int MODE>
-__global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt, float *map_part,
+template <typename X, int S>
+__global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args a, Plan pl, const float *carry, float *map_part,
                                                               float *par_part) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
     __shared__ float4 s_step[kWaves][Q][CH];         // dt, dt * u, dy; then the step's sums g . b, A . w, c . h
-    // b and c; then the wave's db and dc, which the workgroup joins while the next block fills the other buffer
-    constexpr int NB = MODE == 0 ? 2 : 1;
-    __shared__ __align__(16) float s_b2[NB][kWaves][Q][NP], s_c2[NB][kWaves][Q][NP];
+    // rows b, c; then the wave's db, dc, which the workgroup joins while the next block fills the other buffer
+    __shared__ __align__(16) float s_maps[2][kWaves][2][Q][NP];
     int buf = 0;
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Wave w;
-    int id = blockIdx.x;
-    const int wg = id % pl.wpg;
-    id /= pl.wpg;
-    w.g = id % a.G;
-    id /= a.G;
-    w.chunk = id % pl.nchunks;
-    w.b = id / pl.nchunks;
+    unsigned id = blockIdx.x;
+    const int wg = (int)(id % (unsigned)pl.wpg);
+    id /= (unsigned)pl.wpg;
+    w.g = (int)(id % (unsigned)a.G);
+    id /= (unsigned)a.G;
+    w.chunk = (int)(id % (unsigned)pl.nchunks);
+    w.b = (int)(id / (unsigned)pl.nchunks);
     const int in_group = wg * kWaves + wv;
-    const bool wave_on = in_group < pl.tpg;          // the last workgroup of a group may have waves to spare
-    set_tile(w, pl, wave_on ? in_group : pl.tpg - 1);
-    if (!wave_on) w.nch = 0;
+    const bool wave_on = in_group < pl.tpg;          // the last workgroup of a group may have waves to spare:
+    const int tile = wave_on ? in_group : pl.tpg - 1;     // they load a channel and use nothing of it
+    w.d0 = w.g * pl.Dg + tile * CH;
+    w.nch = wave_on ? min(CH, pl.Dg - tile * CH) : 0;
     set_time(w, pl, a.T, a.lengths);
-    if (MODE == 1 && !wave_on) return;
-    const int load_ch = wave_on ? w.nch : 1;         // a spare wave loads one channel and uses nothing of it
-    const int c = lane / S, s = lane % S, ec = lane % CH;
+    const int load_ch = wave_on ? w.nch : 1;
+    Lane<S> me;
+    me.init(a.a, a.N, w);
+    const int c = me.c, s = me.s, ec = lane % CH;
     const bool e_on = ec < w.nch;
     const int ed = w.d0 + min(ec, load_ch - 1);
-    const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f;
-    const float skip = (MODE == 0 && a.skip) ? a.skip[ed] : 0.f;
-    float a2[4], g[4] = {0.f, 0.f, 0.f, 0.f}, dts = 0.f;
-    load_rates(a.a, a.N, w, c, s, a2);
-    if (MODE == 0) {
-        if (pl.nchunks > 1) {
-            if (wave_on) {
-                const float4 v = reinterpret_cast<const float4 *>(carry)[lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile)];
-                g[0] = v.x; g[1] = v.y; g[2] = v.z; g[3] = v.w;
-            }
-        } else if (a.dfinal) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (c < w.nch && 4 * s + k < a.N) g[k] = a.dfinal[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k];
-        }
+    const float bias = a.delta_bias ? a.delta_bias[ed] : 0.f, skip = a.skip ? a.skip[ed] : 0.f;
+    float g[4] = {0.f, 0.f, 0.f, 0.f};
+    if (pl.nchunks > 1) {
+        if (me.on) unpack(*reinterpret_cast<const float4 *>(carry + ((long)w.b * pl.nchunks + w.chunk) * a.D * NP + me.at), g);
+    } else if (a.dfinal) {
+        me.load(a.dfinal, w, a.D, a.N, g);
     }
     Rows<X, S> pu, pd, pz, pg, pdu, pdd, pdz;
-    Maps<X, S> pb, pc;
+    Maps<X, S> mb, mc;
+    mb.init(a.b, a.b_stride, w.b, w.g);
+    mc.init(a.c, a.c_stride, w.b, w.g);
+    pu.init(a.u, a.u_stride, w.b, w.d0, load_ch);
     pd.init(a.delta, a.delta_stride, w.b, w.d0, load_ch);
-    pc.init(a.c, a.c_stride, w.b, w.g, a.N);
     if (a.dy) pg.init(a.dy, a.dy_stride, w.b, w.d0, load_ch);
     if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, load_ch);
-    if (MODE == 0) {
-        pu.init(a.u, a.u_stride, w.b, w.d0, load_ch);
-        pb.init(a.b, a.b_stride, w.b, w.g, a.N);
-        if (a.du) pdu.init(a.du, a.du_stride, w.b, w.d0, load_ch);
-        if (a.ddelta) pdd.init(a.ddelta, a.ddelta_stride, w.b, w.d0, load_ch);
-        if (a.dz) pdz.init(a.dz, a.dz_stride, w.b, w.d0, load_ch);
-    }
-    X ru[E], rd[E], rz[E], rg[E], rb[S], rc[S];
+    if (a.du) pdu.init(a.du, a.du_stride, w.b, w.d0, load_ch);
+    if (a.ddelta) pdd.init(a.ddelta, a.ddelta_stride, w.b, w.d0, load_ch);
+    if (a.dz) pdz.init(a.dz, a.dz_stride, w.b, w.d0, load_ch);
+    const float *ckpt = a.reserve + (long)w.b * pl.nblk * a.D * NP + me.at;
+    X ru[E], rd[E], rz[E], rg[E];
     float4 rh;
     auto request = [&](int t0) {
         const int left = w.tv - t0;
         pd.load(rd, t0, left);
+        pu.load(ru, t0, left);
         if (a.dy) pg.load(rg, t0, left);
-        pc.load(rc, t0, left);
         if (a.z) pz.load(rz, t0, left);
-        if (MODE == 0) {
-            pu.load(ru, t0, left);
-            pb.load(rb, t0, left);
-            rh = reinterpret_cast<const float4 *>(a.reserve)[lane_slot(pl, w.b, t0 / Q, pl.nblk, w.tile)];
-        }
+        mb.load(t0, left, a.N, pl.quads);
+        mc.load(t0, left, a.N, pl.quads);
+        rh = *reinterpret_cast<const float4 *>(ckpt + (long)(t0 / Q) * a.D * NP);
     };
     // sums over all steps: dA by state, dskip and ddelta_bias by channel
     float dA[4] = {0.f, 0.f, 0.f, 0.f}, dskip = 0.f, dbias = 0.f;
@@ -509,56 +579,52 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
     for (int t0 = last; t0 >= w.t_lo; t0 -= Q) {
         float u[E], z[E], out[E], dt[E], dy[E], slope[E], gate[E];
         const int left = w.tv - t0;                  // steps of this block that exist (Q or more: all)
-        auto &s_b = s_b2[buf], &s_c = s_c2[buf];
+        auto &s_map = s_maps[buf][wv];
         wave_sync();
+        // (a block that is there in full, in a wave whose channels all exist, needs no selection)
         const bool full = left >= Q && w.nch == CH;
         auto stage = [&](auto full) {
 #pragma unroll
             for (int j = 0; j < E; ++j) {
                 const int et = lane / CH + j * S;
                 const bool on = full.value || (e_on && et < left);
-                u[j] = (MODE == 0 && on) ? to_float(ru[j]) : 0.f;
-                z[j] = a.z ? to_float(rz[j]) : 0.f;
+                u[j] = on ? to_float(ru[j]) : 0.f;
                 out[j] = (a.dy && on) ? to_float(rg[j]) : 0.f;
                 const float raw = to_float(rd[j]) + bias;
-                dt[j] = on ? (a.softplus ? softplus(raw) : raw) : 0.f;
-                slope[j] = a.softplus ? sigmoid(raw) : 1.f;
-                gate[j] = a.z ? sigmoid(z[j]) : 1.f;
-                dy[j] = (a.z && on) ? out[j] * z[j] * gate[j] : out[j];
+                dt[j] = raw;
+                slope[j] = 1.f;
+                if (a.softplus) softplus_slope(raw, dt[j], slope[j]);
+                if (!full.value) dt[j] = on ? dt[j] : 0.f;
+                dy[j] = out[j];
+                if (a.z) {
+                    z[j] = to_float(rz[j]);
+                    gate[j] = sigmoid(z[j]);
+                    dy[j] *= z[j] * gate[j];
+                    if (!full.value) dy[j] = on ? dy[j] : 0.f;
+                }
                 s_step[wv][et][ec] = make_float4(dt[j], dt[j] * u[j], dy[j], 0.f);
             }
         };
         if (full) stage(std::true_type{});
         else stage(std::false_type{});
-        if (MODE == 0) pb.to_lds(&s_b[wv][0][0], rb, a.N, left);
-        pc.to_lds(&s_c[wv][0][0], rc, a.N, left);
-        const float h0[4] = {rh.x, rh.y, rh.z, rh.w};
+        mb.to_lds(&s_map[0][0][0], left, a.N);
+        mc.to_lds(&s_map[1][0][0], left, a.N);
+        const float h0[4] = {me.on ? rh.x : 0.f, me.on ? rh.y : 0.f, me.on ? rh.z : 0.f, me.on ? rh.w : 0.f};
         if (t0 > w.t_lo) request(t0 - Q);
         wave_sync();
-        if (MODE == 1) {
-            for (int i = min(left, Q) - 1; i >= 0; --i) {
-                const float4 v = s_step[wv][i][c];
-                const float4 c4 = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
-                const float cc[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) g[k] = __builtin_amdgcn_exp2f(v.x * a2[k]) * __builtin_fmaf(v.z, cc[k], g[k]);
-                dts += v.x;
-            }
-            continue;
-        }
         float blkA[4] = {0.f, 0.f, 0.f, 0.f};
         auto fetch = [&](int i, bool reverse) {
             StepIn in;
             in.v = s_step[wv][i][c];
-            in.b = *reinterpret_cast<const float4 *>(&s_b[wv][i][4 * s]);
-            if (reverse) in.c = *reinterpret_cast<const float4 *>(&s_c[wv][i][4 * s]);
+            in.b = *reinterpret_cast<const float4 *>(&s_map[0][i][4 * s]);
+            if (reverse) in.c = *reinterpret_cast<const float4 *>(&s_map[1][i][4 * s]);
             return in;
         };
         auto advance = [&](const StepIn &in, const float (&from)[4], float (&to)[4], float (&decay)[4]) {
             const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                decay[k] = __builtin_amdgcn_exp2f(in.v.x * a2[k]);
+                decay[k] = __builtin_amdgcn_exp2f(in.v.x * me.a2[k]);
                 to[k] = __builtin_fmaf(decay[k], from[k], in.v.y * bb[k]);
             }
         };
@@ -598,7 +664,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
                         ch[r] = __builtin_fmaf(cc[k], h[i][k], ch[r]);
                         g[k] = gt * decay[i][k];
                         const float wk = g[k] * (i ? h[i ? i - 1 : 0][k] : h0[k]);
-                        aw[r] = __builtin_fmaf(wk, a2[k], aw[r]);
+                        aw[r] = __builtin_fmaf(wk, me.a2[k], aw[r]);
                         blkA[k] = __builtin_fmaf(wk, v.x, blkA[k]);
                     }
                     gb[r] = pin(sum_parts<S>(gb[r]));
@@ -613,8 +679,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
                 // quarter q of the wave has, in part s of each of its channels, the sums of state 4 s + value of q
                 const int n = 4 * s + 2 * ((lane >> 4) & 1) + (lane >> 5);
                 write_four<16 / S>(lane % 16 / S, [&](int which, auto pick) {
-                    s_b[wv][first + i0 + which][n] = pick(sb);
-                    s_c[wv][first + i0 + which][n] = pick(sc);
+                    s_map[0][first + i0 + which][n] = pick(sb);
+                    s_map[1][first + i0 + which][n] = pick(sc);
                 });
             }
         };
@@ -641,46 +707,50 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
         for (int k = 0; k < 4; ++k) dA[k] += blkA[k];
         wave_sync();
         float bs = 0.f, bb = 0.f;
-        auto finish = [&](auto full) {
+        float4 sums[E];
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                const int et = lane / CH + j * S;
-                if (!full.value && (!e_on || et >= left)) continue;
-                const float4 r = s_step[wv][et][ec];
-                const float du = __builtin_fmaf(r.x, dt[j], skip * dy[j]);
-                const float dd = __builtin_fmaf(r.x, u[j], kLn2 * r.y) * slope[j];
+        for (int j = 0; j < E; ++j) sums[j] = s_step[wv][lane / CH + j * S][ec];
+        auto finish = [&](auto full) {
+            auto each = [&](auto f) {
+#pragma unroll
+                for (int j = 0; j < E; ++j)
+                    if (full.value || (e_on && lane / CH + j * S < left)) f(j);
+            };
+            each([&](int j) {
+                const float du = __builtin_fmaf(sums[j].x, dt[j], skip * dy[j]);
                 bs = __builtin_fmaf(dy[j], u[j], bs);
-                bb += dd;
                 if (a.du) pdu.store(t0, j, du);
+            });
+            each([&](int j) {
+                const float dd = __builtin_fmaf(sums[j].x, u[j], kLn2 * sums[j].y) * slope[j];
+                bb += dd;
                 if (a.ddelta) pdd.store(t0, j, dd);
-                if (a.dz)
-                    pdz.store(t0, j, out[j] * __builtin_fmaf(skip, u[j], r.z) * gate[j] * __builtin_fmaf(z[j], 1.f - gate[j], 1.f));
-            }
+            });
+            if (a.dz)
+                each([&](int j) {
+                    pdz.store(t0, j, out[j] * __builtin_fmaf(skip, u[j], sums[j].z) * gate[j] * __builtin_fmaf(z[j], 1.f - gate[j], 1.f));
+                });
         };
         if (full) finish(std::true_type{});
         else finish(std::false_type{});
         dskip += bs;
         dbias += bb;
         if (map_part) {
-            // the four waves' sums of this block, joined: map_part[b][g][workgroup][t][db, dc][NP]
+            // the four waves' sums of this block, joined: map_part[b][g][workgroup][db, dc][t][NP]
             lds_barrier();
-            float *to = map_part + ((((long)w.b * a.G + w.g) * pl.wpg + wg) * a.T + t0) * 2 * NP;
-            for (int e = threadIdx.x; e < 2 * Q * NP; e += 64 * kWaves) {
-                const int t = e / (2 * NP), n = e % (2 * NP);
-                if (t0 + t >= w.tv) break;
-                float v = 0.f;
+            const long row = (((long)w.b * a.G + w.g) * pl.wpg + wg) * 2;
+            const int n = min(left, Q) * NP;
+            for (int m = 0; m < 2; ++m) {
+                float *to = map_part + ((row + m) * a.T + t0) * NP;
+                for (int e = threadIdx.x; e < n; e += 64 * kWaves) {
+                    float v = 0.f;
 #pragma unroll
-                for (int q = 0; q < kWaves; ++q) v += n < NP ? s_b[q][t][n] : s_c[q][t][n - NP];
-                to[e] = v;
+                    for (int q = 0; q < kWaves; ++q) v += (&s_maps[buf][q][m][0][0])[e];
+                    to[e] = v;
+                }
             }
-            buf ^= NB - 1;
+            buf ^= 1;
         }
-    }
-    if (MODE == 1) {
-        const long at = lane_slot(pl, w.b, w.chunk, pl.nchunks, w.tile);
-        reinterpret_cast<float4 *>(carry)[at] = make_float4(g[0], g[1], g[2], g[3]);
-        sdt[at] = dts;
-        return;
     }
     // rows behind the end
     for (int t = max(w.t_lo, w.tv) + lane / CH; t < w.t_hi; t += S) {
@@ -690,11 +760,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
         if (a.ddelta) static_cast<X *>(a.ddelta)[w.b * a.ddelta_stride[0] + t * a.ddelta_stride[1] + ed] = zero;
         if (a.dz) static_cast<X *>(a.dz)[w.b * a.dz_stride[0] + t * a.dz_stride[1] + ed] = zero;
     }
-    if (a.dinitial && w.chunk == 0 && c < w.nch) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (4 * s + k < a.N) a.dinitial[((long)w.b * a.D + w.d0 + c) * a.N + 4 * s + k] = g[k];
-    }
+    if (a.dinitial && w.chunk == 0) me.store(a.dinitial, w, a.D, a.N, g);
     if (!par_part) return;
     // par_part[b, chunk][dA (D, N) | dskip (D) | ddelta_bias (D)]
     float *to = par_part + ((long)w.b * pl.nchunks + w.chunk) * a.D * (a.N + 2);
@@ -714,25 +780,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
     }
 }
 
-// db, dc (B, T, G, N) from map_part[b][g][workgroup][t][db, dc][NP], the workgroups in order; zeros behind the end.
+// db, dc (B, T, G, N) from map_part[b][g][workgroup][db, dc][t][NP], the workgroups in order; zeros behind the end.
 template <typename X>
 __global__ __launch_bounds__(256) void scan_map_grad_kernel(tgru_scan_args a, Plan pl, const float *__restrict__ map_part) {
-    const int NP = 4 * pl.S;
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;         // (b, g, t, db | dc, n)
-    const int e = (int)(id % (2 * NP));
-    const long row = id / (2 * NP);
-    const int t = (int)(row % a.T);
-    const long bg = row / a.T;
-    const int n = e % NP;
+    const long per = (long)a.T * pl.NP, id = (long)blockIdx.x * 256 + threadIdx.x;         // (b, g, db | dc, t, n)
+    const long part = id / per, bg = part >> 1;
+    const int e = (int)(id - part * per), t = e / pl.NP, n = e - t * pl.NP;
     if (bg >= (long)a.B * a.G || n >= a.N) return;
-    const int b = (int)(bg / a.G), g = (int)(bg % a.G);
+    const int b = (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
     float v = 0.f;
     if (t < clamped_length(a.lengths, b, a.T)) {
-        const float *p = map_part + (bg * pl.wpg * a.T + t) * 2 * NP + e;
-        const long step = (long)a.T * 2 * NP;
-        for (int q = 0; q < pl.wpg; ++q) v += p[q * step];
+        const float *p = map_part + (bg * pl.wpg * 2 + (part & 1)) * per + e;
+        for (int q = 0; q < pl.wpg; ++q) v += p[q * 2 * per];
     }
-    X *to = static_cast<X *>(e < NP ? a.db : a.dc);
+    X *to = static_cast<X *>((part & 1) ? a.dc : a.db);
     if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
 }
 
@@ -815,28 +876,32 @@ __global__ __launch_bounds__(64) void scan_step_kernel(tgru_scan_step_args a, in
         if (4 * s + k < a.N) a.state_out[so + k] = h[k];
 }
 
-int lanes_per_channel(int N) {
-    int S = 1;
-    while (4 * S < N) S <<= 1;
-    return S;
+// States with padding: a power of two, 8 at least (with four a lane of scan_bwd_kernel would have too much of the work
+// that is per channel in its registers).
+int padded_states(int N) {
+    int n = 8;
+    while (n < N) n <<= 1;
+    return n;
 }
 
-// Chunks of time: as many as fill the chip, none where the channels alone do.
+// Chunks of time: as many as fill the chip, none where the channels alone do.  A chunked pass computes the recurrence
+// twice, so it pays from about three chunks on; four blocks a chunk at least.
 Plan make_plan(int B, int T, int D, int N, int G) {
     Plan p;
-    p.S = lanes_per_channel(N);
-    p.CH = 64 / p.S;
+    p.NP = padded_states(N);
+    p.CH = 256 / p.NP;
     p.Dg = D / G;
     p.tpg = (p.Dg + p.CH - 1) / p.CH;
     p.tiles = p.tpg * G;
     p.wpg = (p.tpg + kWaves - 1) / kWaves;
     p.nblk = (T + Q - 1) / Q;
     p.nchunks = 1;
+    p.quads = 0;
     const long waves = (long)B * p.tiles;
-    if (waves < 768) {
-        const long want = (2048 + waves - 1) / waves, most = (p.nblk + 3) / 4;      // four blocks a chunk at least
+    if (waves < kEnoughWaves) {
+        const long want = (kFullWaves + waves - 1) / waves, most = (p.nblk + 3) / 4;
         const long n = want < most ? want : most;
-        if (n >= 3) p.nchunks = (int)n;                 // a chunked pass does the work twice
+        if (n >= 3) p.nchunks = (int)n;
     }
     p.chunk = (p.nblk + p.nchunks - 1) / p.nchunks * Q;
     p.nchunks = (T + p.chunk - 1) / p.chunk;
@@ -846,21 +911,25 @@ Plan make_plan(int B, int T, int D, int N, int G) {
 int scan_dims(int B, int T, int D, int N, int G) {
     if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || N > TGRU_SCAN_MAX_STATES || D % G) return TGRU_E_DIMS;
     if (T > (1 << 30) || D > (1 << 26)) return TGRU_E_DIMS;
+    // the widest launches' workgroup numbers, and their waves', in 31 bits
     const Plan p = make_plan(B, T, D, N, G);
-    // workgroup numbers of the widest launch (the maps' gradients: one thread per (b, t, g, db | dc, state)) in 31 bits
-    if ((double)B * p.tiles * p.nchunks >= 2147483648.0 || (double)B * T * G * 8 * p.S / 256 >= 2147483647.0) return TGRU_E_DIMS;
+    if ((double)B * p.nchunks * G * p.wpg * kWaves >= 2147483648.0 || (double)B * D * p.NP / 64 >= 2147483647.0 ||
+        (double)B * T * G * 2 * p.NP / 256 >= 2147483647.0 || (double)T * p.NP >= 2147483648.0)
+        return TGRU_E_DIMS;
     return TGRU_OK;
 }
 
-struct Workspace { size_t carry, sdt, map, par, total; };       // offsets in floats
+size_t ckpt_floats(const Plan &p, int B, int D) { return (size_t)B * p.nblk * D * p.NP; }
+
+struct Workspace { size_t carry, sdt, map, par, total; };       // offsets in floats, each a multiple of 4
 Workspace workspace_of(const Plan &p, int B, int T, int D, int N, int G, bool backward) {
     Workspace w;
     size_t off = 0;
-    const size_t lanes = p.nchunks > 1 ? (size_t)B * p.nchunks * p.tiles * 64 : 0;
-    w.carry = off; off += 4 * lanes;
-    w.sdt = off; off += lanes;
-    w.map = off; off += backward ? (size_t)B * G * p.wpg * T * 8 * p.S : 0;
-    w.par = off; off += backward ? (size_t)B * p.nchunks * D * (N + 2) : 0;
+    auto take = [&](size_t n) { const size_t at = off; off += (n + 3) & ~(size_t)3; return at; };
+    w.carry = take(p.nchunks > 1 ? (size_t)B * p.nchunks * D * p.NP : 0);
+    w.sdt = take(p.nchunks > 1 ? (size_t)B * p.nchunks * D : 0);
+    w.map = take(backward ? (size_t)B * G * p.wpg * T * 2 * p.NP : 0);
+    w.par = take(backward ? (size_t)B * p.nchunks * D * (N + 2) : 0);
     w.total = off;
     return w;
 }
@@ -868,19 +937,24 @@ Workspace workspace_of(const Plan &p, int B, int T, int D, int N, int G, bool ba
 #define TGRU_DONE() do { if (hipGetLastError() != hipSuccess) return TGRU_E_LAUNCH; } while (0)
 
 template <typename X, int S>
-int run_scan(const tgru_scan_args &a, const Plan &pl, bool backward, hipStream_t s) {
+int run_scan(const tgru_scan_args &a, bool backward, hipStream_t s) {
+    Plan pl = make_plan(a.B, a.T, a.D, a.N, a.G);
+    auto quads = [&](const void *p, const int64_t *st) {
+        return (uintptr_t)p % (4 * sizeof(X)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
+    };
+    pl.quads = a.N % 4 == 0 && quads(a.b, a.b_stride) && quads(a.c, a.c_stride);
     const Workspace ws = workspace_of(pl, a.B, a.T, a.D, a.N, a.G, backward);
     float *carry = a.workspace + ws.carry, *sdt = a.workspace + ws.sdt;
-    const dim3 join((unsigned)(a.B * pl.tiles)), block(64 * kWaves);
+    const dim3 run((unsigned)(((long)a.B * pl.nchunks * pl.tiles + kWaves - 1) / kWaves)), block(64 * kWaves);
+    const dim3 join((unsigned)(((long)a.B * a.D * pl.NP + 63) / 64));
     if (!backward) {
-        const dim3 grid((unsigned)(((long)a.B * pl.nchunks * pl.tiles + kWaves - 1) / kWaves));
         if (pl.nchunks > 1) {
-            TGRU_LAUNCH((scan_fwd_kernel<X, S, 1>), grid, block, 0, s, a, pl, carry, sdt);
+            TGRU_LAUNCH((scan_fwd_kernel<X, S, 1>), run, block, 0, s, a, pl, carry, sdt);
             TGRU_DONE();
-            TGRU_LAUNCH((scan_join_kernel<S>), join, dim3(64), 0, s, a.a, a.initial_state, pl, a.D, a.N, 0, carry, sdt);
+            TGRU_LAUNCH(scan_join_kernel, join, dim3(64), 0, s, a.a, a.initial_state, pl, a.B, a.D, a.N, 0, carry, sdt);
             TGRU_DONE();
         }
-        TGRU_LAUNCH((scan_fwd_kernel<X, S, 0>), grid, block, 0, s, a, pl, carry, sdt);
+        TGRU_LAUNCH((scan_fwd_kernel<X, S, 0>), run, block, 0, s, a, pl, carry, sdt);
         TGRU_DONE();
         return TGRU_OK;
     }
@@ -888,15 +962,15 @@ int run_scan(const tgru_scan_args &a, const Plan &pl, bool backward, hipStream_t
     float *map = (a.db || a.dc) ? a.workspace + ws.map : nullptr;
     float *par = (a.da || a.dskip || a.ddelta_bias) ? a.workspace + ws.par : nullptr;
     if (pl.nchunks > 1) {
-        TGRU_LAUNCH((scan_bwd_kernel<X, S, 1>), grid, block, 0, s, a, pl, carry, sdt, nullptr, nullptr);
+        TGRU_LAUNCH((scan_back_kernel<X, S>), run, block, 0, s, a, pl, carry, sdt);
         TGRU_DONE();
-        TGRU_LAUNCH((scan_join_kernel<S>), join, dim3(64), 0, s, a.a, a.dfinal, pl, a.D, a.N, 1, carry, sdt);
+        TGRU_LAUNCH(scan_join_kernel, join, dim3(64), 0, s, a.a, a.dfinal, pl, a.B, a.D, a.N, 1, carry, sdt);
         TGRU_DONE();
     }
-    TGRU_LAUNCH((scan_bwd_kernel<X, S, 0>), grid, block, 0, s, a, pl, carry, sdt, map, par);
+    TGRU_LAUNCH((scan_bwd_kernel<X, S>), grid, block, 0, s, a, pl, carry, map, par);
     TGRU_DONE();
     if (map) {
-        const long n = (long)a.B * a.G * a.T * 8 * S;
+        const long n = (long)a.B * a.G * a.T * 2 * pl.NP;
         TGRU_LAUNCH((scan_map_grad_kernel<X>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, pl, map);
         TGRU_DONE();
     }
@@ -910,13 +984,12 @@ int run_scan(const tgru_scan_args &a, const Plan &pl, bool backward, hipStream_t
 }
 
 template <typename X>
-int run_scan_lanes(const tgru_scan_args &a, const Plan &pl, bool backward, hipStream_t s) {
-    switch (pl.S) {
-    case 1: return run_scan<X, 1>(a, pl, backward, s);
-    case 2: return run_scan<X, 2>(a, pl, backward, s);
-    case 4: return run_scan<X, 4>(a, pl, backward, s);
-    case 8: return run_scan<X, 8>(a, pl, backward, s);
-    default: return run_scan<X, 16>(a, pl, backward, s);
+int run_scan_states(const tgru_scan_args &a, bool backward, hipStream_t s) {
+    switch (padded_states(a.N)) {
+    case 8: return run_scan<X, 2>(a, backward, s);
+    case 16: return run_scan<X, 4>(a, backward, s);
+    case 32: return run_scan<X, 8>(a, backward, s);
+    default: return run_scan<X, 16>(a, backward, s);
     }
 }
 
@@ -925,9 +998,8 @@ int scan_call(const tgru_scan_args *a, bool backward, hipStream_t s) {
     if (int rc = scan_dims(a->B, a->T, a->D, a->N, a->G)) return rc;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     if (!a->u || !a->delta || !a->b || !a->c || !a->a) return TGRU_E_NULL;
-    const Plan pl = make_plan(a->B, a->T, a->D, a->N, a->G);
     if (backward ? !a->reserve || (a->dz && !a->z) : !a->y) return TGRU_E_NULL;
-    if ((backward || pl.nchunks > 1) && !a->workspace) return TGRU_E_NULL;
+    if (!a->workspace && tgru_scan_workspace_bytes(a->B, a->T, a->D, a->N, a->G, backward)) return TGRU_E_NULL;
     auto wide = [](const void *p, const int64_t *stride) { return p && (stride[1] < 0 || stride[1] >= kMaxRowStride); };
     if (wide(a->u, a->u_stride) || wide(a->delta, a->delta_stride) || wide(a->z, a->z_stride) || wide(a->b, a->b_stride) ||
         wide(a->c, a->c_stride) || wide(a->y, a->y_stride) || wide(a->dy, a->dy_stride) || wide(a->du, a->du_stride) ||
@@ -935,9 +1007,9 @@ int scan_call(const tgru_scan_args *a, bool backward, hipStream_t s) {
         return TGRU_E_DIMS;
     if (((uintptr_t)a->reserve & 15) || ((uintptr_t)a->workspace & 15)) return TGRU_E_ALIGN;
     if (int rc = check_device()) return rc;
-    if (a->dtype == TGRU_DTYPE_F32) return run_scan_lanes<float>(*a, pl, backward, s);
-    if (a->dtype == TGRU_DTYPE_BF16) return run_scan_lanes<__bf16>(*a, pl, backward, s);
-    return run_scan_lanes<_Float16>(*a, pl, backward, s);
+    if (a->dtype == TGRU_DTYPE_F32) return run_scan_states<float>(*a, backward, s);
+    if (a->dtype == TGRU_DTYPE_BF16) return run_scan_states<__bf16>(*a, backward, s);
+    return run_scan_states<_Float16>(*a, backward, s);
 }
 
 template <typename X, int S>
@@ -950,7 +1022,9 @@ int run_scan_step(const tgru_scan_step_args &a, hipStream_t s) {
 
 template <typename X>
 int run_scan_step_lanes(const tgru_scan_step_args &a, hipStream_t s) {
-    switch (lanes_per_channel(a.N)) {
+    int S = 1;
+    while (4 * S < a.N) S <<= 1;
+    switch (S) {
     case 1: return run_scan_step<X, 1>(a, s);
     case 2: return run_scan_step<X, 2>(a, s);
     case 4: return run_scan_step<X, 4>(a, s);
@@ -968,14 +1042,12 @@ extern "C" {
 
 size_t tgru_scan_reserve_bytes(int B, int T, int D, int N, int G) {
     if (scan_dims(B, T, D, N, G) != TGRU_OK) return 0;
-    const Plan p = make_plan(B, T, D, N, G);
-    return (size_t)B * p.nblk * p.tiles * 64 * 4 * sizeof(float);
+    return ckpt_floats(make_plan(B, T, D, N, G), B, D) * sizeof(float);
 }
 
 size_t tgru_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward) {
     if (scan_dims(B, T, D, N, G) != TGRU_OK) return 0;
-    const Plan p = make_plan(B, T, D, N, G);
-    return workspace_of(p, B, T, D, N, G, backward != 0).total * sizeof(float);
+    return workspace_of(make_plan(B, T, D, N, G), B, T, D, N, G, backward != 0).total * sizeof(float);
 }
 
 int tgru_scan_forward(const tgru_scan_args *a, tgru_stream_t stream) { return scan_call(a, false, (hipStream_t)stream); }

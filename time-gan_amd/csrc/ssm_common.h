@@ -22,24 +22,20 @@ __device__ __forceinline__ float sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
 }
 
-// log(1 + exp(v)) = max(v, 0) + log1p(exp(-|v|)) with log1p(e) = 2 atanh(e / (2 + e)): e is in [0, 1], so the atanh
-// argument s is in [0, 1/3] and its Taylor series in s^2 <= 1/9 is cut after nine terms (the next one is below
-// 9^-9 / 19, 2^-32 of the result).  Unlike log2(1 + e) on the hardware unit it keeps its relative precision where the
-// result is small -- step sizes of 0.001 are v = -6.9.
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|) in [0, 1].  log1p(e) = log(w) + (e - (w - 1)) for the rounded
+// sum w = 1 + e: what the sum lost is added back (divided by w it would be exact to first order; w is in [1, 2] and the
+// term below half a step of w), so the result keeps its relative precision where it is small -- step sizes of 0.001 are
+// v = -6.9.  The slope is the sigmoid of v.  Measured against 64 bits: 10 half steps at v in [-10, 0), 2.4 above, 18 at
+// -15, nearly all of it the rounding of exp2's argument.
+__device__ __forceinline__ void softplus_slope(float v, float &value, float &slope) {
+    const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(v)), w = 1.f + e, r = __builtin_amdgcn_rcpf(w);
+    value = fmaxf(v, 0.f) + __builtin_fmaf(kLn2, __builtin_amdgcn_logf(w), e - (w - 1.f));
+    slope = v < 0.f ? e * r : r;
+}
 __device__ __forceinline__ float softplus(float v) {
-    const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(v));
-    const float s = e * __builtin_amdgcn_rcpf(2.f + e);
-    const float q = s * s;
-    float p = 1.f / 17.f;
-    p = __builtin_fmaf(p, q, 1.f / 15.f);
-    p = __builtin_fmaf(p, q, 1.f / 13.f);
-    p = __builtin_fmaf(p, q, 1.f / 11.f);
-    p = __builtin_fmaf(p, q, 1.f / 9.f);
-    p = __builtin_fmaf(p, q, 1.f / 7.f);
-    p = __builtin_fmaf(p, q, 1.f / 5.f);
-    p = __builtin_fmaf(p, q, 1.f / 3.f);
-    p = __builtin_fmaf(p, q, 1.f);
-    return __builtin_fmaf(2.f * s, p, fmaxf(v, 0.f));
+    float value, slope;
+    softplus_slope(v, value, slope);
+    return value;
 }
 
 __device__ __forceinline__ int clamped_length(const int32_t *lengths, int b, int T) {
