@@ -195,30 +195,6 @@ struct Maps {
 struct StepIn { float4 v, b, c; };
 __device__ __forceinline__ void ahead() { __builtin_amdgcn_sched_barrier(0); }
 
-// x, kept where it is: the compiler may not move the computation of x into a branch behind this point.
-__device__ __forceinline__ float pin(float x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-
-// Writes four steps' values, which all lanes of a channel (or all replicas of a sum) hold, with one write per lane that
-// stores step `which` of 0..3; lanes beyond the first four repeat a value.  `n` replicas: fewer than four write several.
-template <int n, typename F>
-__device__ __forceinline__ void write_four(int replica, F &&write) {
-    if constexpr (n >= 4) {
-        write(replica & 3, [&](const float (&v)[4]) {
-            const float lo = (replica & 1) ? v[1] : v[0], hi = (replica & 1) ? v[3] : v[2];
-            return (replica & 2) ? hi : lo;
-        });
-    } else if constexpr (n == 2) {
-        write(replica, [&](const float (&v)[4]) { return replica ? v[1] : v[0]; });
-        write(2 + replica, [&](const float (&v)[4]) { return replica ? v[3] : v[2]; });
-    } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) write(r, [&](const float (&v)[4]) { return v[r]; });
-    }
-}
-
 // A wave of the passes whose waves are independent of each other; false where there is none.
 __device__ __forceinline__ bool place_wave(Wave &w, const tgru_scan_args &a, const Plan &pl) {
     const unsigned id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -234,7 +210,9 @@ __device__ __forceinline__ bool place_wave(Wave &w, const tgru_scan_args &a, con
     return true;
 }
 
-// This lane's four states: where they are in a row of carry or ckpt, and their rates to base 2 per unit of dt.
+// This lane's four states: where they are in a row of carry or ckpt, and their rates to base 2 per unit of dt.  Steps behind
+// a sequence's end are staged as dt = 0, which leaves a state as it is, exactly: exp2(0 a2) = 1 for every finite a2 (an
+// infinite one is taken as 3e38: the same decay to nothing for every dt > 0).
 template <int S>
 struct Lane {
     int c, s;                        // channel of the wave, part of the channel
@@ -247,7 +225,10 @@ struct Lane {
         on = c < w.nch;
         at = (long)(w.d0 + (on ? c : 0)) * (4 * S) + 4 * s;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a2[k] = has(k, N) ? rates[(long)(w.d0 + c) * N + 4 * s + k] * kLog2e : 0.f;
+        for (int k = 0; k < 4; ++k) {
+            const float v = has(k, N) ? rates[(long)(w.d0 + c) * N + 4 * s + k] * kLog2e : 0.f;
+            a2[k] = __builtin_isinf(v) ? __builtin_copysignf(3.0e38f, v) : v;
+        }
     }
     __device__ __forceinline__ bool has(int k, int N) const { return on && 4 * s + k < N; }
     // from / to a (B, D, N) tensor
@@ -353,18 +334,18 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
             if (MODE == 1) dts += in.v.x;
             else s_y[i][lane] = __builtin_fmaf(in.c.x, h[0], __builtin_fmaf(in.c.y, h[1], __builtin_fmaf(in.c.z, h[2], in.c.w * h[3])));
         };
-        if (left >= Q) {
+        auto steps = [&](auto count) {
             StepIn next = fetch(0);
 #pragma unroll
-            for (int i = 0; i < Q; ++i) {
+            for (int i = 0; i < count.value; ++i) {
                 const StepIn in = next;
-                if (i + 1 < Q) next = fetch(i + 1);
+                if (i + 1 < count.value) next = fetch(i + 1);
                 ahead();
                 step(i, in);
             }
-        } else {                                     // the sequence ends inside this block
-            for (int i = 0; i < left; ++i) step(i, fetch(i));
-        }
+        };
+        if (left > Q / 2) steps(std::integral_constant<int, Q>{});
+        else for (int i = 0; i < left; ++i) step(i, fetch(i));
         if (MODE == 0) {
             wave_sync();
             auto finish = [&](auto full) {
@@ -456,17 +437,13 @@ __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a
             for (int k = 0; k < 4; ++k) g[k] = __builtin_amdgcn_exp2f(in.v.x * me.a2[k]) * __builtin_fmaf(in.v.y, cc[k], g[k]);
             dts += in.v.x;
         };
-        if (left >= Q) {
-            StepIn next = fetch(Q - 1);
+        StepIn next = fetch(Q - 1);
 #pragma unroll
-            for (int i = Q - 1; i >= 0; --i) {
-                const StepIn in = next;
-                if (i > 0) next = fetch(i - 1);
-                ahead();
-                step(in);
-            }
-        } else {
-            for (int i = left - 1; i >= 0; --i) step(fetch(i));
+        for (int i = Q - 1; i >= 0; --i) {
+            const StepIn in = next;
+            if (i > 0) next = fetch(i - 1);
+            ahead();
+            step(in);
         }
     }
     if (!me.on) return;
@@ -629,7 +606,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
             }
         };
         // steps first .. first + R - 1 of the block, from state h0 in front of them; `next` is step `first`
-        auto part = [&](auto whole, auto first_, const float (&h0)[4], StepIn next) {
+        auto part = [&](auto first_, const float (&h0)[4], StepIn next) {
             constexpr int first = first_.value;
             float decay[R][4], h[R][4];
 #pragma unroll
@@ -637,72 +614,52 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
                 const StepIn in = next;
                 next = i + 1 < R ? fetch(first + i + 1, false) : fetch(first + R - 1, true);
                 ahead();
-                if (!whole.value && first + i >= left) continue;
                 advance(in, i ? h[i ? i - 1 : 0] : h0, h[i], decay[i]);
             }
-            // from the last step to the first, four at a time: their sums are written together
+            // from the last step to the first
 #pragma unroll
-            for (int i0 = R - 4; i0 >= 0; i0 -= 4) {
-                float gb[4], aw[4], ch[4], sb[4], sc[4];
+            for (int i = R - 1; i >= 0; --i) {
+                const StepIn in = next;
+                if (i > 0) next = fetch(first + i - 1, true);
+                ahead();
+                float bb[4], cc[4], db[4], dc[4], gb = 0.f, aw = 0.f, ch = 0.f;
+                unpack(in.b, bb);
+                unpack(in.c, cc);
 #pragma unroll
-                for (int r = 3; r >= 0; --r) {
-                    const int i = i0 + r;
-                    gb[r] = aw[r] = ch[r] = sb[r] = sc[r] = 0.f;
-                    const StepIn in = next;
-                    if (i > 0) next = fetch(first + i - 1, true);
-                    ahead();
-                    if (!whole.value && first + i >= left) continue;
-                    const float4 v = in.v;
-                    const float bb[4] = {in.b.x, in.b.y, in.b.z, in.b.w}, cc[4] = {in.c.x, in.c.y, in.c.z, in.c.w};
-                    float db[4], dc[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float gt = __builtin_fmaf(v.z, cc[k], g[k]);
-                        dc[k] = v.z * h[i][k];
-                        db[k] = v.y * gt;
-                        gb[r] = __builtin_fmaf(gt, bb[k], gb[r]);
-                        ch[r] = __builtin_fmaf(cc[k], h[i][k], ch[r]);
-                        g[k] = gt * decay[i][k];
-                        const float wk = g[k] * (i ? h[i ? i - 1 : 0][k] : h0[k]);
-                        aw[r] = __builtin_fmaf(wk, me.a2[k], aw[r]);
-                        blkA[k] = __builtin_fmaf(wk, v.x, blkA[k]);
-                    }
-                    gb[r] = pin(sum_parts<S>(gb[r]));
-                    aw[r] = pin(sum_parts<S>(aw[r]));
-                    ch[r] = pin(sum_parts<S>(ch[r]));
-                    sb[r] = pin(sum_channels<S>(db));
-                    sc[r] = pin(sum_channels<S>(dc));
+                for (int k = 0; k < 4; ++k) {
+                    const float gt = __builtin_fmaf(in.v.z, cc[k], g[k]);
+                    dc[k] = in.v.z * h[i][k];
+                    db[k] = in.v.y * gt;
+                    gb = __builtin_fmaf(gt, bb[k], gb);
+                    ch = __builtin_fmaf(cc[k], h[i][k], ch);
+                    g[k] = gt * decay[i][k];
+                    const float wk = g[k] * (i ? h[i ? i - 1 : 0][k] : h0[k]);
+                    aw = __builtin_fmaf(wk, me.a2[k], aw);
+                    blkA[k] = __builtin_fmaf(wk, in.v.x, blkA[k]);
                 }
-                write_four<S>(s, [&](int which, auto pick) {
-                    s_step[wv][first + i0 + which][c] = make_float4(pick(gb), pick(aw), pick(ch), 0.f);
-                });
+                // (all lanes that hold a sum write it, the same value to the same place: no selection, no branch)
+                s_step[wv][first + i][c] = make_float4(sum_parts<S>(gb), sum_parts<S>(aw), sum_parts<S>(ch), 0.f);
                 // quarter q of the wave has, in part s of each of its channels, the sums of state 4 s + value of q
                 const int n = 4 * s + 2 * ((lane >> 4) & 1) + (lane >> 5);
-                write_four<16 / S>(lane % 16 / S, [&](int which, auto pick) {
-                    s_map[0][first + i0 + which][n] = pick(sb);
-                    s_map[1][first + i0 + which][n] = pick(sc);
-                });
+                s_map[0][first + i][n] = sum_channels<S>(db);
+                s_map[1][first + i][n] = sum_channels<S>(dc);
             }
         };
         // The states of R steps are kept in registers: the second half of the block first, from a state that is carried
         // through the first half and forgotten again.
-        auto block = [&](auto whole) {
-            if (whole.value || left > R) {
-                float hm[4] = {h0[0], h0[1], h0[2], h0[3]}, decay[4];
-                StepIn next = fetch(0, false);
+        if (left > R) {
+            float hm[4] = {h0[0], h0[1], h0[2], h0[3]}, decay[4];
+            StepIn next = fetch(0, false);
 #pragma unroll
-                for (int i = 0; i < R; ++i) {
-                    const StepIn in = next;
-                    next = fetch(i + 1, false);
-                    ahead();
-                    advance(in, hm, hm, decay);
-                }
-                part(whole, std::integral_constant<int, R>{}, hm, next);
+            for (int i = 0; i < R; ++i) {
+                const StepIn in = next;
+                next = fetch(i + 1, false);
+                ahead();
+                advance(in, hm, hm, decay);
             }
-            part(whole, std::integral_constant<int, 0>{}, h0, fetch(0, false));
-        };
-        if (left >= Q) block(std::true_type{});
-        else block(std::false_type{});
+            part(std::integral_constant<int, R>{}, hm, next);
+        }
+        part(std::integral_constant<int, 0>{}, h0, fetch(0, false));
 #pragma unroll
         for (int k = 0; k < 4; ++k) dA[k] += blkA[k];
         wave_sync();
