@@ -39,9 +39,6 @@ constexpr int R = Q / 2;             // steps whose states the backward pass kee
 constexpr int kWaves = 4;            // per workgroup
 constexpr int64_t kMaxRowStride = TGRU_SCAN_MAX_ROW_STRIDE;
 
-// make_plan's limits, in waves: enough of them without chunks, and what chunks are cut for.
-constexpr long kEnoughWaves = 768, kFullWaves = 4096;
-
 struct Plan {                        // how a pass is cut up; made on the host
     int NP, CH, Dg;                  // states with padding (8 .. 64), channels per wave, channels per group
     int tpg, tiles, wpg;             // waves per group, per sequence and chunk; workgroups per group (scan_bwd_kernel)
@@ -258,6 +255,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
     auto &s_y = s_ys[MODE == 0 ? wv : 0];
     Wave w;
     if (!place_wave(w, a, pl)) return;
+    if (MODE == 1 && w.chunk == pl.nchunks - 1) return;                 // nobody goes on from it
     Lane<S> me;
     me.init(a.a, a.N, w);
     const int ec = lane % CH, ed = w.d0 + min(ec, w.nch - 1);           // this lane's channel when it works per channel
@@ -385,7 +383,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a
     auto &s_step = s_steps[wv];
     auto &s_map = s_maps[wv];
     Wave w;
-    if (!place_wave(w, a, pl)) return;
+    if (!place_wave(w, a, pl) || w.chunk == 0) return;
     Lane<S> me;
     me.init(a.a, a.N, w);
     const int ec = lane % CH;
@@ -451,7 +449,8 @@ __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a
     if (me.s == 0) sdt[((long)w.b * pl.nchunks + w.chunk) * a.D + w.d0 + me.c] = dts;
 }
 
-// Joins the chunks: carry[chunk] becomes what enters the chunk.  `edge`: (B, D, N) entering the first chunk in the
+// Joins the chunks: carry[chunk] becomes what enters the chunk.  (What the last one in the order of the pass would hand on
+// was not computed: its slot is read, and what comes of it is not used.)  `edge`: (B, D, N) entering the first chunk in the
 // order of the pass (the initial state forward, the final state's gradient backward), or null.  One thread per state.
 __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const float *edge, Plan pl, int B, int D, int N, int backward,
                                                        float *carry, const float *sdt) {
@@ -841,9 +840,18 @@ int padded_states(int N) {
     return n;
 }
 
-// Chunks of time: as many as fill the chip, none where the channels alone do.  A chunked pass computes the recurrence
-// twice, so it pays from about three chunks on; four blocks a chunk at least.
-Plan make_plan(int B, int T, int D, int N, int G) {
+// What a pass of `waves` waves over `steps` steps takes, in us: cost[k - 1] is one step's time with k waves on each of the
+// chip's 1024 SIMDs, of which it holds `most` -- so whole rounds of them and what is left over.
+double pass_time(long waves, long steps, const double *cost, int most) {
+    const long round = 1024L * most, rest = waves % round;
+    return steps * (waves / round * cost[most - 1] + (rest ? cost[(rest + 1023) / 1024 - 1] : 0.));
+}
+
+// Chunks of time: the number that the times measured below give the shortest pass for.  A chunk more costs the main pass
+// nothing but blocks cut short; the pass in front does more of its work again (all chunks but one), and with the joining
+// costs two launches.  Measured (16 states, us a step): one sequence more or less than a round matters most -- 1280 and
+// 2048 waves of the backward pass take the same 510 us for 1024 steps, 2560 take 797.
+Plan make_plan(int B, int T, int D, int N, int G, bool backward) {
     Plan p;
     p.NP = padded_states(N);
     p.CH = 256 / p.NP;
@@ -852,16 +860,22 @@ Plan make_plan(int B, int T, int D, int N, int G) {
     p.tiles = p.tpg * G;
     p.wpg = (p.tpg + kWaves - 1) / kWaves;
     p.nblk = (T + Q - 1) / Q;
-    p.nchunks = 1;
     p.quads = 0;
+    static const double fwd[] = {.133, .165, .21, .30}, fwd_front[] = {.09, .124, .165, .225}, bwd[] = {.36, .503},
+                        bwd_front[] = {.10, .135, .185, .26};
     const long waves = (long)B * p.tiles;
-    if (waves < kEnoughWaves) {
-        const long want = (kFullWaves + waves - 1) / waves, most = (p.nblk + 3) / 4;
-        const long n = want < most ? want : most;
-        if (n >= 3) p.nchunks = (int)n;
+    double best = 0.;
+    p.nchunks = 1;
+    p.chunk = p.nblk * Q;
+    for (int n = 1; n <= 128 && n <= p.nblk; n += n < 8 ? 1 : n / 4) {
+        const int chunk = (p.nblk + n - 1) / n * Q, real = (T + chunk - 1) / chunk;
+        double time = backward ? pass_time(waves * real, chunk, bwd, 2) : pass_time(waves * real, chunk, fwd, 4);
+        if (real > 1) time += 10. + pass_time(waves * (real - 1), chunk, backward ? bwd_front : fwd_front, 4);
+        if (n > 1 && time >= best) continue;
+        best = time;
+        p.nchunks = real;
+        p.chunk = chunk;
     }
-    p.chunk = (p.nblk + p.nchunks - 1) / p.nchunks * Q;
-    p.nchunks = (T + p.chunk - 1) / p.chunk;
     return p;
 }
 
@@ -869,8 +883,8 @@ int scan_dims(int B, int T, int D, int N, int G) {
     if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || N > TGRU_SCAN_MAX_STATES || D % G) return TGRU_E_DIMS;
     if (T > (1 << 30) || D > (1 << 26)) return TGRU_E_DIMS;
     // the widest launches' workgroup numbers, and their waves', in 31 bits
-    const Plan p = make_plan(B, T, D, N, G);
-    if ((double)B * p.nchunks * G * p.wpg * kWaves >= 2147483648.0 || (double)B * D * p.NP / 64 >= 2147483647.0 ||
+    const Plan p = make_plan(B, T, D, N, G, false);
+    if ((double)B * 128 * G * p.wpg * kWaves >= 2147483648.0 || (double)B * D * p.NP / 64 >= 2147483647.0 ||
         (double)B * T * G * 2 * p.NP / 256 >= 2147483647.0 || (double)T * p.NP >= 2147483648.0)
         return TGRU_E_DIMS;
     return TGRU_OK;
@@ -895,7 +909,7 @@ Workspace workspace_of(const Plan &p, int B, int T, int D, int N, int G, bool ba
 
 template <typename X, int S>
 int run_scan(const tgru_scan_args &a, bool backward, hipStream_t s) {
-    Plan pl = make_plan(a.B, a.T, a.D, a.N, a.G);
+    Plan pl = make_plan(a.B, a.T, a.D, a.N, a.G, backward);
     auto quads = [&](const void *p, const int64_t *st) {
         return (uintptr_t)p % (4 * sizeof(X)) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
     };
@@ -999,12 +1013,12 @@ extern "C" {
 
 size_t tgru_scan_reserve_bytes(int B, int T, int D, int N, int G) {
     if (scan_dims(B, T, D, N, G) != TGRU_OK) return 0;
-    return ckpt_floats(make_plan(B, T, D, N, G), B, D) * sizeof(float);
+    return ckpt_floats(make_plan(B, T, D, N, G, false), B, D) * sizeof(float);
 }
 
 size_t tgru_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward) {
     if (scan_dims(B, T, D, N, G) != TGRU_OK) return 0;
-    return workspace_of(make_plan(B, T, D, N, G), B, T, D, N, G, backward != 0).total * sizeof(float);
+    return workspace_of(make_plan(B, T, D, N, G, backward != 0), B, T, D, N, G, backward != 0).total * sizeof(float);
 }
 
 int tgru_scan_forward(const tgru_scan_args *a, tgru_stream_t stream) { return scan_call(a, false, (hipStream_t)stream); }
