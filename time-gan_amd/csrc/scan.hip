@@ -736,54 +736,59 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
     }
 }
 
-// db, dc (B, T, G, N) from map_part[b][g][workgroup][db, dc][t][NP], the workgroups in order; zeros behind the end.
+// The gradients that several workgroups of scan_bwd_kernel have a share of; everything is added in a fixed order.
+//   workgroups [0, map_blocks): db, dc (B, T, G, N) from map_part[b][g][workgroup][db, dc][t][NP]; zeros behind the end
+//   the others: da, dskip, ddelta_bias from the rows of par_part[rows][D (N + 2)], 64 columns x 4 groups of rows each
 template <typename X>
-__global__ __launch_bounds__(256) void scan_map_grad_kernel(tgru_scan_args a, Plan pl, const float *__restrict__ map_part) {
-    const long per = (long)a.T * pl.NP, id = (long)blockIdx.x * 256 + threadIdx.x;         // (b, g, db | dc, t, n)
-    const long part = id / per, bg = part >> 1;
-    const int e = (int)(id - part * per), t = e / pl.NP, n = e - t * pl.NP;
-    if (bg >= (long)a.B * a.G || n >= a.N) return;
-    const int b = (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
-    float v = 0.f;
-    if (t < clamped_length(a.lengths, b, a.T)) {
-        const float *p = map_part + (bg * pl.wpg * 2 + (part & 1)) * per + e;
-        for (int q = 0; q < pl.wpg; ++q) v += p[q * 2 * per];
+__global__ __launch_bounds__(256) void scan_grads_kernel(tgru_scan_args a, Plan pl, const float *__restrict__ map_part, unsigned map_blocks,
+                                                         const float *__restrict__ par_part) {
+    if (blockIdx.x < map_blocks) {
+        const long per = (long)a.T * pl.NP, id = (long)blockIdx.x * 256 + threadIdx.x;     // (b, g, db | dc, t, n)
+        const long part = id / per, bg = part >> 1;
+        const int e = (int)(id - part * per), t = e / pl.NP, n = e - t * pl.NP;
+        if (bg >= (long)a.B * a.G || n >= a.N) return;
+        const int b = (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
+        float v = 0.f;
+        if (t < clamped_length(a.lengths, b, a.T)) {
+            const float *p = map_part + (bg * pl.wpg * 2 + (part & 1)) * per + e;
+#pragma unroll 8
+            for (int q = 0; q < pl.wpg; ++q) v += p[q * 2 * per];
+        }
+        X *to = static_cast<X *>((part & 1) ? a.dc : a.db);
+        if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
+        return;
     }
-    X *to = static_cast<X *>((part & 1) ? a.dc : a.db);
-    if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
-}
-
-// da, dskip, ddelta_bias from par_part[rows][D (N + 2)]: 64 columns x 4 groups of rows per workgroup, joined in order.
-__global__ __launch_bounds__(256) void scan_param_grad_kernel(const float *__restrict__ part, int rows, int D, int N, float *da,
-                                                              float *dskip, float *dbias) {
     __shared__ float red[4][64];
-    const int c = threadIdx.x & 63, grp = threadIdx.x >> 6;
-    const long cols = (long)D * (N + 2), col = (long)blockIdx.x * 64 + c;
-    const int per = (rows + 3) / 4, r0 = grp * per, r1 = min(rows, r0 + per);
+    const int c = threadIdx.x & 63, grp = threadIdx.x >> 6, rows = a.B * pl.nchunks;
+    const long cols = (long)a.D * (a.N + 2), col = (long)(blockIdx.x - map_blocks) * 64 + c;
+    const int each = (rows + 3) / 4, r0 = grp * each, r1 = min(rows, r0 + each);
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (col < cols) {
         int r = r0;
         for (; r + 3 < r1; r += 4)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) s[q] += part[(long)(r + q) * cols + col];
-        for (; r < r1; ++r) s[0] += part[(long)r * cols + col];
+            for (int q = 0; q < 4; ++q) s[q] += par_part[(long)(r + q) * cols + col];
+        for (; r < r1; ++r) s[0] += par_part[(long)r * cols + col];
     }
     red[grp][c] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
     if (grp != 0 || col >= cols) return;
     const float v = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-    const long dn = (long)D * N;
-    if (col < dn) { if (da) da[col] = v; }
-    else if (col < dn + D) { if (dskip) dskip[col - dn] = v; }
-    else if (dbias) dbias[col - dn - D] = v;
+    const long dn = (long)a.D * a.N;
+    if (col < dn) { if (a.da) a.da[col] = v; }
+    else if (col < dn + a.D) { if (a.dskip) a.dskip[col - dn] = v; }
+    else if (a.ddelta_bias) a.ddelta_bias[col - dn - a.D] = v;
 }
 
-// One token: a wave takes CH channels of one row.  Rows with one slot are taken in order by the first one's wave.
+// One token: a wave takes CH channels of one row.  Bound by the states, read and written once: four of them a lane, in one
+// load where N is a multiple of 4.  Rows with one slot are taken in order by the first one's wave.
 template <typename X, int S>
-__global__ __launch_bounds__(64) void scan_step_kernel(tgru_scan_step_args a, int tpg, int tiles) {
+__global__ __launch_bounds__(64 * kWaves) void scan_step_kernel(tgru_scan_step_args a, int tpg, int tiles, int quads) {
     constexpr int CH = 64 / S;
-    const int lane = threadIdx.x, c = lane / S, s = lane % S;
-    const int row0 = blockIdx.x / tiles, flat = blockIdx.x - row0 * tiles;
+    const int lane = threadIdx.x & 63, c = lane / S, s = lane % S;
+    const unsigned id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row0 = (int)(id / (unsigned)tiles), flat = (int)(id - (unsigned)row0 * (unsigned)tiles);
+    if (row0 >= a.B) return;
     const int grp = flat / tpg, Dg = a.D / a.G, first = (flat - grp * tpg) * CH;
     const bool on = c < Dg - first;
     const int d = grp * Dg + first + (on ? c : 0);
@@ -792,44 +797,56 @@ __global__ __launch_bounds__(64) void scan_step_kernel(tgru_scan_step_args a, in
         if (on && s == 0) static_cast<X *>(a.y)[row0 * a.y_stride + d] = from_float<X>(0.f);
         return;
     }
-    if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
-    float h[4], a2[4];
-    const long so = ((long)slot * a.D + d) * a.N + 4 * s;
+    const int n0 = min(4 * s, quads ? a.N - 4 : a.N - 1);               // parts without states read the last ones
+    const long so = ((long)slot * a.D + d) * a.N, ao = (long)d * a.N;
+    // four values of a row of N, zeros beyond it
+    auto four = [&](const auto *p, float (&v)[4]) {
+        using E = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+        struct alignas(4 * sizeof(E)) Pack4 { E v[4]; };
+        if (quads) {
+            const Pack4 q = *reinterpret_cast<const Pack4 *>(p + n0);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const bool has = 4 * s + k < a.N;
-        const long at = has ? k : -4 * s;             // a state that does not exist reads the channel's first one
-        h[k] = has ? a.state[so + at] : 0.f;
-        a2[k] = has ? a.a[(long)d * a.N + 4 * s + k] * kLog2e : 0.f;
-    }
+            for (int k = 0; k < 4; ++k) v[k] = 4 * s < a.N ? to_float(q.v[k]) : 0.f;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = 4 * s + k < a.N ? to_float(p[min(4 * s + k, a.N - 1)]) : 0.f;
+        }
+    };
+    float h[4], a2[4];
+    four(a.state + so, h);
+    four(a.a + ao, a2);
     const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+    __builtin_amdgcn_sched_barrier(0);       // all of that is on its way while the search waits for its own loads
+    if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
     for (int row = row0; row < a.B;) {
+        float b[4], m[4];
+        four(static_cast<const X *>(a.b) + row * a.b_stride[0] + grp * a.b_stride[1], b);
+        four(static_cast<const X *>(a.c) + row * a.c_stride[0] + grp * a.c_stride[1], m);
         const float u = to_float(static_cast<const X *>(a.u)[row * a.u_stride + d]);
         const float raw = to_float(static_cast<const X *>(a.delta)[row * a.delta_stride + d]) + bias;
-        const float dt = a.softplus ? softplus(raw) : raw;
-        const X *b = static_cast<const X *>(a.b) + row * a.b_stride[0] + grp * a.b_stride[1];
-        const X *m = static_cast<const X *>(a.c) + row * a.c_stride[0] + grp * a.c_stride[1];
+        const float z = a.z ? to_float(static_cast<const X *>(a.z)[row * a.z_stride + d]) : 0.f;
+        const float dt = a.softplus ? softplus(raw) : raw, t = dt * kLog2e;
         float y = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int n = min(4 * s + k, a.N - 1);
-            const float bb = 4 * s + k < a.N ? to_float(b[n]) : 0.f, cc = 4 * s + k < a.N ? to_float(m[n]) : 0.f;
-            h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * a2[k]), h[k], dt * u * bb);
-            y = __builtin_fmaf(cc, h[k], y);
+            h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(t * a2[k]), h[k], dt * u * b[k]);
+            y = __builtin_fmaf(m[k], h[k], y);
         }
         y = __builtin_fmaf(skip, u, sum_parts<S>(y));
-        if (a.z) {
-            const float z = to_float(static_cast<const X *>(a.z)[row * a.z_stride + d]);
-            y *= z * sigmoid(z);
-        }
+        if (a.z) y *= z * sigmoid(z);
         if (on && s == 0) static_cast<X *>(a.y)[row * a.y_stride + d] = from_float<X>(y);
         if (!a.slots) break;
         row = find_slot(a.slots, row + 1, a.B, slot);
     }
-    if (!on) return;
+    if (!on || 4 * s >= a.N) return;
+    float *to = a.state_out + so + 4 * s;
+    if (quads) {
+        *reinterpret_cast<float4 *>(to) = make_float4(h[0], h[1], h[2], h[3]);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (4 * s + k < a.N) a.state_out[so + k] = h[k];
+        for (int k = 0; k < 4; ++k)
+            if (4 * s + k < a.N) to[k] = h[k];
+    }
 }
 
 // States with padding: a power of two, 8 at least (with four a lane of scan_bwd_kernel would have too much of the work
@@ -885,7 +902,7 @@ int scan_dims(int B, int T, int D, int N, int G) {
     // the widest launches' workgroup numbers, and their waves', in 31 bits
     const Plan p = make_plan(B, T, D, N, G, false);
     if ((double)B * 128 * G * p.wpg * kWaves >= 2147483648.0 || (double)B * D * p.NP / 64 >= 2147483647.0 ||
-        (double)B * T * G * 2 * p.NP / 256 >= 2147483647.0 || (double)T * p.NP >= 2147483648.0)
+        (double)B * T * G * 2 * p.NP / 256 + (double)D * (N + 2) / 64 >= 2147483646.0 || (double)T * p.NP >= 2147483648.0)
         return TGRU_E_DIMS;
     return TGRU_OK;
 }
@@ -940,15 +957,10 @@ int run_scan(const tgru_scan_args &a, bool backward, hipStream_t s) {
     }
     TGRU_LAUNCH((scan_bwd_kernel<X, S>), grid, block, 0, s, a, pl, carry, map, par);
     TGRU_DONE();
-    if (map) {
-        const long n = (long)a.B * a.G * a.T * 2 * pl.NP;
-        TGRU_LAUNCH((scan_map_grad_kernel<X>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a, pl, map);
-        TGRU_DONE();
-    }
-    if (par) {
-        const long cols = (long)a.D * (a.N + 2);
-        TGRU_LAUNCH(scan_param_grad_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, s, par, a.B * pl.nchunks, a.D, a.N,
-                    a.da, a.dskip, a.ddelta_bias);
+    if (map || par) {
+        const unsigned maps = map ? (unsigned)(((long)a.B * a.G * a.T * 2 * pl.NP + 255) / 256) : 0;
+        const unsigned pars = par ? (unsigned)(((long)a.D * (a.N + 2) + 63) / 64) : 0;
+        TGRU_LAUNCH((scan_grads_kernel<X>), dim3(maps + pars), dim3(256), 0, s, a, pl, map, maps, par);
         TGRU_DONE();
     }
     return TGRU_OK;
@@ -986,7 +998,12 @@ int scan_call(const tgru_scan_args *a, bool backward, hipStream_t s) {
 template <typename X, int S>
 int run_scan_step(const tgru_scan_step_args &a, hipStream_t s) {
     const int CH = 64 / S, tpg = (a.D / a.G + CH - 1) / CH, tiles = tpg * a.G;
-    TGRU_LAUNCH((scan_step_kernel<X, S>), dim3((unsigned)((long)a.B * tiles)), dim3(64), 0, s, a, tpg, tiles);
+    auto ok = [](const void *p, size_t align) { return (uintptr_t)p % align == 0; };
+    const int quads = a.N % 4 == 0 && ok(a.state, 16) && ok(a.state_out, 16) && ok(a.a, 16) && ok(a.b, 4 * sizeof(X)) &&
+                      ok(a.c, 4 * sizeof(X)) && a.b_stride[0] % 4 == 0 && a.b_stride[1] % 4 == 0 && a.c_stride[0] % 4 == 0 &&
+                      a.c_stride[1] % 4 == 0;
+    TGRU_LAUNCH((scan_step_kernel<X, S>), dim3((unsigned)(((long)a.B * tiles + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0, s, a, tpg,
+                tiles, quads);
     TGRU_DONE();
     return TGRU_OK;
 }

@@ -12,7 +12,7 @@ namespace tgru {
 namespace ssm {
 
 constexpr int kConvThreads = 256;
-constexpr int kRows = 8;             // rows requested together
+constexpr int kRows = 8, kRowsBack = 4;      // rows requested together
 
 template <typename X, int VEC>
 struct alignas(sizeof(X) * VEC) Pack { X v[VEC]; };
@@ -61,13 +61,26 @@ __device__ __forceinline__ void input_row(const tgru_conv_args &a, const Place &
     for (int i = 0; i < VEC; ++i) v[i] = to_float(r.v[i]);
 }
 
+// The taps of VEC channels lie next to each other; with packs they start on 16 bytes.
 template <int K, int VEC>
 __device__ __forceinline__ void load_taps(const float *weight, const float *bias, int d, float (&w)[K][VEC], float (&b)[VEC]) {
+    float flat[K * VEC];
+    const float *from = weight + (long)d * K;
+    if constexpr (VEC >= 4) {
+#pragma unroll
+        for (int j = 0; j < K * VEC / 4; ++j) {
+            const float4 v = reinterpret_cast<const float4 *>(from)[j];
+            flat[4 * j] = v.x; flat[4 * j + 1] = v.y; flat[4 * j + 2] = v.z; flat[4 * j + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < K * VEC; ++j) flat[j] = from[j];
+    }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
         b[i] = bias ? bias[d + i] : 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][i] = weight[(long)(d + i) * K + k];
+        for (int k = 0; k < K; ++k) w[k][i] = flat[i * K + k];
     }
 }
 
@@ -143,22 +156,22 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(tgru_conv_args a
         for (int k = 1; k < K; ++k) input_row<X, K, VEC>(a, p, p.t0 - K + k, win[k]);
     }
     const long xo = p.b * a.x_stride[0] + p.d, go = p.b * a.dy_stride[0] + p.d, dxo = p.b * a.dx_stride[0] + p.d;
-    for (int t = p.t0; t < p.t1 + K - 1; t += kRows) {
-        Pack<X, VEC> rx[kRows], rg[kRows];
+    for (int t = p.t0; t < p.t1 + K - 1; t += kRowsBack) {
+        Pack<X, VEC> rx[kRowsBack], rg[kRowsBack];
 #pragma unroll
-        for (int r = 0; r < kRows; ++r)
+        for (int r = 0; r < kRowsBack; ++r)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) rx[r].v[i] = rg[r].v[i] = from_float<X>(0.f);
         if (t < te) {
 #pragma unroll
-            for (int r = 0; r < kRows; ++r) rx[r] = load_pack<X, VEC>(a.x, xo + (long)min(t + r, te - 1) * a.x_stride[1]);
+            for (int r = 0; r < kRowsBack; ++r) rx[r] = load_pack<X, VEC>(a.x, xo + (long)min(t + r, te - 1) * a.x_stride[1]);
             if (a.dy) {
 #pragma unroll
-                for (int r = 0; r < kRows; ++r) rg[r] = load_pack<X, VEC>(a.dy, go + (long)min(t + r, te - 1) * a.dy_stride[1]);
+                for (int r = 0; r < kRowsBack; ++r) rg[r] = load_pack<X, VEC>(a.dy, go + (long)min(t + r, te - 1) * a.dy_stride[1]);
             }
         }
 #pragma unroll
-        for (int r = 0; r < kRows; ++r) {
+        for (int r = 0; r < kRowsBack; ++r) {
             const int now = t + r, s = now - (K - 1);
             const bool on = now < te, mine = now < p.t1;
             float dx[VEC];
@@ -252,13 +265,14 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
         if (on) store_pack<X, VEC>(a.y, row0 * a.y_stride + d, zero);
         return;
     }
-    if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
     float w[K][VEC], bias[VEC], win[K][VEC];
     load_taps<K, VEC>(a.weight, a.bias, d, w, bias);
     const long so = (long)slot * (K - 1) * a.D + d;
     Pack<X, VEC> st[K > 1 ? K - 1 : 1];
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) st[k] = load_pack<X, VEC>(a.state, so + (long)k * a.D);
+    __builtin_amdgcn_sched_barrier(0);       // all of that is on its way while the search waits for its own loads
+    if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
 #pragma unroll
     for (int k = 0; k < K - 1; ++k)
 #pragma unroll
@@ -286,13 +300,16 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
 }
 
 // Steps per run: as long as the launch still has about `waves` waves, because the K - 1 rows around a run are read
-// twice; 8 at least (one group of loads), 64 at most.
+// twice; 8 at least (one group of loads), 64 at most.  16-byte packs need few waves to fill the memory's queues, single
+// elements many.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 53 us with 2048 waves (5.1 TB/s), 58 with
+// 4096, 71 with 8192; backward 107 us with 2048 (four rows at a time; 150 with eight, which leaves one wave per SIMD fewer),
+// 111 with 1024, 120 with 4096.  7 x 1531 steps of 1003 channels, single elements: 12 us with 8192, 16 with 2048.
 int conv_run_len(int B, int T, int nvec, long waves) {
     int len = 64;
     while (len > 8 && (long)B * ((T + len - 1) / len) * nvec < waves * 64) len >>= 1;
     return len;
 }
-constexpr long kConvWavesFwd = 8192, kConvWavesBwd = 2048;
+constexpr long kConvWaves = 2048, kConvWavesSingle = 8192;
 
 bool multiple_of(long v, long m) { return v % m == 0; }
 
@@ -302,7 +319,7 @@ bool conv_packs(const tgru_conv_args &a, bool backward) {
     auto ok = [&](const void *p, const int64_t *st) {
         return !p || (((uintptr_t)p & 15) == 0 && (!st || (multiple_of(st[0], vec) && multiple_of(st[1], vec))));
     };
-    bool v = a.D % vec == 0 && ok(a.x, a.x_stride) && ok(a.initial_state, nullptr);
+    bool v = a.D % vec == 0 && ok(a.weight, nullptr) && ok(a.x, a.x_stride) && ok(a.initial_state, nullptr);
     if (!backward) return v && ok(a.y, a.y_stride) && ok(a.final_state, nullptr);
     return v && ok(a.dy, a.dy_stride) && ok(a.dx, a.dx_stride) && ok(a.dfinal, nullptr) && ok(a.dinitial, nullptr);
 }
@@ -312,7 +329,7 @@ int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
     const bool packs = conv_packs(a, backward);
     const int vec = packs ? 16 / (int)sizeof(X) : 1;
     const int nvec = a.D / vec;
-    const int len = conv_run_len(a.B, a.T, nvec, backward ? kConvWavesBwd : kConvWavesFwd), runs = (a.T + len - 1) / len;
+    const int len = conv_run_len(a.B, a.T, nvec, packs || backward ? kConvWaves : kConvWavesSingle), runs = (a.T + len - 1) / len;
     const dim3 grid((unsigned)(((long)a.B * runs * nvec + kConvThreads - 1) / kConvThreads)), block(kConvThreads);
     constexpr int VEC = 16 / (int)sizeof(X);
     if (!backward) {
@@ -335,7 +352,7 @@ template <typename X, int K>
 int run_conv_step(const tgru_conv_step_args &a, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(X);
     auto ok = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
-    const bool packs = a.D % VEC == 0 && ok(a.x) && ok(a.y) && ok(a.state) && ok(a.state_out) &&
+    const bool packs = a.D % VEC == 0 && ok(a.weight) && ok(a.x) && ok(a.y) && ok(a.state) && ok(a.state_out) &&
                        multiple_of(a.x_stride, VEC) && multiple_of(a.y_stride, VEC);
     const int nvec = packs ? a.D / VEC : a.D, nblk = (nvec + 63) / 64;
     const dim3 grid((unsigned)((long)a.B * nblk)), block(64);
@@ -389,7 +406,7 @@ size_t tgru_conv_backward_workspace_bytes(int B, int T, int D, int K) {
     size_t rows = 0;
     for (int vec = 1; vec <= 8; vec *= 2) {
         if (D % vec) break;
-        const int len = conv_run_len(B, T, D / vec, kConvWavesBwd);
+        const int len = conv_run_len(B, T, D / vec, kConvWaves);
         const size_t r = (size_t)B * ((T + len - 1) / len);
         if (r > rows) rows = r;
     }
