@@ -7,12 +7,13 @@
 // requested together; only the K - 1 rows in front of a run are read twice (out of the cache: the run before has them).
 // Lanes run over channels first, so a wave's loads are consecutive.
 #include "ssm_common.h"
+#include <type_traits>
 
 namespace tgru {
 namespace ssm {
 
 constexpr int kConvThreads = 256;
-constexpr int kRows = 8, kRowsBack = 4;      // rows requested together
+constexpr int kRows = 8, kRowsBack = 2;      // rows requested together
 
 template <typename X, int VEC>
 struct alignas(sizeof(X) * VEC) Pack { X v[VEC]; };
@@ -137,7 +138,8 @@ __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(tgru_conv_args a
 //     dx_s = sum_k w[k] dpre_{s+K-1-k},   dw[k] = sum_t dpre_t x_{t-K+1+k},   dbias = sum_t dpre_t.
 // A run looks K - 1 steps past its end (dx there needs them; they count towards dw in the run that owns them).  The
 // sums over a run's steps stay in registers; every run leaves one row (K + 1, D) of them, which a second kernel adds
-// up in a fixed order.
+// up in a fixed order.  Registers decide here (taps, two windows and the sums are 140 floats a lane): two rows at a time
+// and the next two on their way took 95 us where four rows without that took 107 and eight 150.
 template <typename X, int K, int VEC>
 __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(tgru_conv_args a, int nvec, int runs, int run_len) {
     const Place p = place_of<VEC>(a, nvec, runs, run_len);
@@ -156,63 +158,78 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(tgru_conv_args a
         for (int k = 1; k < K; ++k) input_row<X, K, VEC>(a, p, p.t0 - K + k, win[k]);
     }
     const long xo = p.b * a.x_stride[0] + p.d, go = p.b * a.dy_stride[0] + p.d, dxo = p.b * a.dx_stride[0] + p.d;
+    Pack<X, VEC> nx[kRowsBack], ng[kRowsBack];      // the next rows, requested while these are worked on
+    auto request = [&](int t) {
+        if (t >= te) return;
+#pragma unroll
+        for (int r = 0; r < kRowsBack; ++r) nx[r] = load_pack<X, VEC>(a.x, xo + (long)min(t + r, te - 1) * a.x_stride[1]);
+        if (a.dy) {
+#pragma unroll
+            for (int r = 0; r < kRowsBack; ++r) ng[r] = load_pack<X, VEC>(a.dy, go + (long)min(t + r, te - 1) * a.dy_stride[1]);
+        }
+    };
+#pragma unroll
+    for (int r = 0; r < kRowsBack; ++r)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) nx[r].v[i] = ng[r].v[i] = from_float<X>(0.f);
+    request(p.t0);
     for (int t = p.t0; t < p.t1 + K - 1; t += kRowsBack) {
         Pack<X, VEC> rx[kRowsBack], rg[kRowsBack];
 #pragma unroll
-        for (int r = 0; r < kRowsBack; ++r)
+        for (int r = 0; r < kRowsBack; ++r) { rx[r] = nx[r]; rg[r] = ng[r]; }
+        request(t + kRowsBack);
+        // Rows that are this run's own, are there, and whose dx is this run's own too need no selection.
+        auto rows = [&](auto inside) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) rx[r].v[i] = rg[r].v[i] = from_float<X>(0.f);
-        if (t < te) {
+            for (int r = 0; r < kRowsBack; ++r) {
+                const int now = t + r, s = now - (K - 1);
+                const bool on = inside.value || now < te, mine = inside.value || (on && now < p.t1);
+                float dx[VEC];
 #pragma unroll
-            for (int r = 0; r < kRowsBack; ++r) rx[r] = load_pack<X, VEC>(a.x, xo + (long)min(t + r, te - 1) * a.x_stride[1]);
-            if (a.dy) {
+                for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-                for (int r = 0; r < kRowsBack; ++r) rg[r] = load_pack<X, VEC>(a.dy, go + (long)min(t + r, te - 1) * a.dy_stride[1]);
-            }
-        }
+                    for (int k = 0; k < K - 1; ++k) { win[k][i] = win[k + 1][i]; dpre[k][i] = dpre[k + 1][i]; }
+                    win[K - 1][i] = to_float(rx[r].v[i]);
+                    float pre = bias[i], d = to_float(rg[r].v[i]);
 #pragma unroll
-        for (int r = 0; r < kRowsBack; ++r) {
-            const int now = t + r, s = now - (K - 1);
-            const bool on = now < te, mine = now < p.t1;
-            float dx[VEC];
+                    for (int k = 0; k < K; ++k) pre = __builtin_fmaf(w[k][i], win[k][i], pre);
+                    if (a.silu) {
+                        const float sg = sigmoid(pre);
+                        d *= sg * __builtin_fmaf(pre, 1.f - sg, 1.f);
+                    }
+                    d = on ? d : 0.f;
+                    dpre[K - 1][i] = d;
+                    if (mine) {
+                        db[i] += d;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
+                        for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(d, win[k][i], dw[k][i]);
+                    }
+                    float v = w[K - 1][i] * dpre[0][i];      // dpre[j] is that of step s + j: tap K - 1 - j
 #pragma unroll
-                for (int k = 0; k < K - 1; ++k) { win[k][i] = win[k + 1][i]; dpre[k][i] = dpre[k + 1][i]; }
-                win[K - 1][i] = to_float(rx[r].v[i]);
-                float pre = bias[i], d = to_float(rg[r].v[i]);
-#pragma unroll
-                for (int k = 0; k < K; ++k) pre = __builtin_fmaf(w[k][i], win[k][i], pre);
-                if (a.silu) {
-                    const float sg = sigmoid(pre);
-                    d *= sg * __builtin_fmaf(pre, 1.f - sg, 1.f);
+                    for (int k = 1; k < K; ++k) v = __builtin_fmaf(w[K - 1 - k][i], dpre[k][i], v);
+                    dx[i] = v;
                 }
-                d = on ? d : 0.f;
-                dpre[K - 1][i] = d;
-                if (mine && on) {
-                    db[i] += d;
-#pragma unroll
-                    for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(d, win[k][i], dw[k][i]);
+                if (inside.value) {
+                    if (a.dx) store_pack<X, VEC>(a.dx, dxo + (long)s * a.dx_stride[1], dx);
+                    continue;
                 }
-                float v = 0.f;      // dpre[j] is that of step s + j: tap K - 1 - j
+                const bool in_run = s >= p.t0 && s < p.t1, before = s < 0 && p.run == 0 && now < p.t1 + K - 1;
+                if (!in_run && !before) continue;
+                const int j = s - p.n + K - 1;      // row of the final state that x_s is
+                if (a.dfinal && j >= 0 && j < K - 1) {
+                    const Pack<X, VEC> f = load_pack<X, VEC>(a.dfinal, ((long)p.b * (K - 1) + j) * a.D + p.d);
 #pragma unroll
-                for (int k = 0; k < K; ++k) v = __builtin_fmaf(w[K - 1 - k][i], dpre[k][i], v);
-                dx[i] = v;
+                    for (int i = 0; i < VEC; ++i) dx[i] += to_float(f.v[i]);
+                }
+                if (in_run) {
+                    if (a.dx) store_pack<X, VEC>(a.dx, dxo + (long)s * a.dx_stride[1], dx);
+                } else if (a.dinitial) {
+                    store_pack<X, VEC>(a.dinitial, ((long)p.b * (K - 1) + s + K - 1) * a.D + p.d, dx);
+                }
             }
-            const bool in_run = s >= p.t0 && s < p.t1, before = s < 0 && p.run == 0 && now < p.t1 + K - 1;
-            if (!in_run && !before) continue;
-            const int j = s - p.n + K - 1;      // row of the final state that x_s is
-            if (a.dfinal && j >= 0 && j < K - 1) {
-                const Pack<X, VEC> f = load_pack<X, VEC>(a.dfinal, ((long)p.b * (K - 1) + j) * a.D + p.d);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) dx[i] += to_float(f.v[i]);
-            }
-            if (in_run) {
-                if (a.dx) store_pack<X, VEC>(a.dx, dxo + (long)s * a.dx_stride[1], dx);
-            } else if (a.dinitial) {
-                store_pack<X, VEC>(a.dinitial, ((long)p.b * (K - 1) + s + K - 1) * a.D + p.d, dx);
-            }
-        }
+        };
+        if (t >= p.t0 + K - 1 && t + kRowsBack <= min(te, p.t1)) rows(std::true_type{});
+        else rows(std::false_type{});
     }
     if (!a.dweight && !a.dbias) return;
     float *part = a.workspace + p.row * (long)(K + 1) * a.D + p.d;
@@ -301,9 +318,9 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
 
 // Steps per run: as long as the launch still has about `waves` waves, because the K - 1 rows around a run are read
 // twice; 8 at least (one group of loads), 64 at most.  16-byte packs need few waves to fill the memory's queues, single
-// elements many.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 53 us with 2048 waves (5.1 TB/s), 58 with
-// 4096, 71 with 8192; backward 107 us with 2048 (four rows at a time; 150 with eight, which leaves one wave per SIMD fewer),
-// 111 with 1024, 120 with 4096.  7 x 1531 steps of 1003 channels, single elements: 12 us with 8192, 16 with 2048.
+// elements many.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 48 us with 2048 waves (5.5 TB/s), 58 with 4096, 71
+// with 8192; backward 95 us with 2048 (4.2 TB/s).  7 x 1531 steps of 1003 channels, single elements: 12 us with 8192, 16
+// with 2048.
 int conv_run_len(int B, int T, int nvec, long waves) {
     int len = 64;
     while (len > 8 && (long)B * ((T + len - 1) / len) * nvec < waves * 64) len >>= 1;
