@@ -190,7 +190,7 @@ def test_ssm_stack_construction(tg):
     s = m.init_state(5)
     assert s.conv[0].shape == (5, 3, 48) and s.scan[1].shape == (5, 48, 16) and s.scan[0].dtype == torch.float32
     m.load_state_dict(tg.SSM(6, 24, 2).state_dict())
-    dt = torch.nn.functional.softplus(m.layers[0].dt_bias)
+    dt = torch.nn.functional.softplus(m.layers[0].dt_bias.detach())
     assert float(dt.min()) > 0.9e-3 and float(dt.max()) < 0.11
     for kw, err in ((dict(bidirectional=True), NotImplementedError), (dict(state_size=65), ValueError), (dict(conv_width=1), ValueError),
                     (dict(dtype=torch.float64), ValueError), (dict(dropout=0.1, num_layers=2), NotImplementedError)):

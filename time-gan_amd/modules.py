@@ -11,6 +11,9 @@ Differences, all output-preserving:
   * pack_padded_sequence / pad_packed_sequence (TimeGANv1.py:56-65) are not materialised: lengths go
     to the kernels, which skip finished sequences and write the padding rows themselves.
 
+`rnn_cls=SSM` builds the networks on the state-space stack of `ssm.py` in the place of the GRU (same constructor and
+forward contract, lengths included; no counterpart in the reference).
+
 `rnn_cls` exists so that the CPU tests and the CPU baseline can build the same networks on
 torch.nn.GRU; with it the forward takes the reference's literal pack -> GRU -> pad route.
 """
@@ -21,6 +24,7 @@ import torch.nn as nn
 
 from .gru import GRU, gru_pair
 from .head import head_apply, head_apply_pair
+from .ssm import SSM
 
 
 class _RecurrentBlock(nn.Module):
@@ -50,8 +54,9 @@ class _RecurrentBlock(nn.Module):
         return self.post(self._run_rnn(getattr(self, self._rnn_name), self.pre(x), t))
 
     def _run_rnn(self, rnn: nn.Module, x: torch.Tensor, t) -> torch.Tensor:
-        if isinstance(rnn, GRU):
-            rnn.cpp_op = False      # (the trainer sums these gradients through the deferred-reduction queue)
+        if isinstance(rnn, (GRU, SSM)):
+            if isinstance(rnn, GRU):
+                rnn.cpp_op = False      # (the trainer sums these gradients through the deferred-reduction queue)
             h, _ = rnn(x, lengths=t)
             if self.padding_value != 0:
                 lens = torch.as_tensor([int(v) for v in t], device=x.device)
@@ -67,7 +72,7 @@ class _RecurrentBlock(nn.Module):
     def _head(self, x: torch.Tensor, ln0, lin1, ln1=None, lin2=None) -> torch.Tensor:
         """[ln0] -> lin1 -> [ln1 -> ReLU -> lin2]: one fused kernel on the GPU path, the torch modules
         themselves on the CPU path (`rnn_cls=torch.nn.GRU`)."""
-        if x.is_cuda and isinstance(getattr(self, self._rnn_name), GRU):
+        if x.is_cuda and isinstance(getattr(self, self._rnn_name), (GRU, SSM)):
             return head_apply(x, ln0, lin1, ln1, lin2)
         h = lin1(x if ln0 is None else ln0(x))
         return h if lin2 is None else lin2(torch.relu(ln1(h)))

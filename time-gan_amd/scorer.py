@@ -16,18 +16,24 @@ import torch
 import torch.nn as nn
 
 from .gru import GRU
+from .ssm import SSM
 from .parallel import all_reduce_grads, broadcast_parameters, dist_sum, multi_rank, shard_bounds
 
 
 class GeneralRNN(nn.Module):
-    """net = RNN (time-major input) -> output sequence -> Linear -> Sigmoid (GeneralRNN.py:27-55)."""
+    """net = RNN (time-major input) -> output sequence -> Linear -> Sigmoid (GeneralRNN.py:27-55).  cfg['rnn']['type']:
+    'gru', or 'ssm' for the state-space stack of ssm.py; `rnn_cls` overrides the class."""
 
-    def __init__(self, cfg: Dict, rnn_cls=GRU):
+    CELLS = {"gru": GRU, "ssm": SSM}
+
+    def __init__(self, cfg: Dict, rnn_cls=None):
         super().__init__()
         c = cfg["rnn"]
         self.type = c["type"]
-        if self.type != "gru":
-            raise NotImplementedError("only the GRU cell runs on the HIP kernels (cfg['rnn']['type'] = 'gru')")
+        if self.type not in self.CELLS:
+            raise NotImplementedError("only the GRU cell and the state-space stack run on the HIP kernels "
+                                      "(cfg['rnn']['type'] = 'gru' or 'ssm')")
+        rnn_cls = rnn_cls or self.CELLS[self.type]
         if str(c.get("bidirectional", "false")).lower() == "true":
             raise NotImplementedError("bidirectional stacks are not used by the reference's call sites")
         self.dim_input = int(c["dim_input"])
