@@ -1,6 +1,8 @@
 """The state-space operators on the GPU against their definition in float64 (ssm_reference.py, which also derives the
 bounds): values and gradients over types, odd sizes, groups, lengths, strides; the one-token forms and their pools; streams
 and graphs; and the `SSM` stack in the places of the GRU."""
+import gc
+
 import pytest
 import torch
 
@@ -366,10 +368,15 @@ def test_captured_and_replayed(tg):
     torch.cuda.current_stream().wait_stream(side)
     torch.cuda.synchronize()
     graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
-    with torch.cuda.graph(graphs[0]):
-        outs = train()
-    with torch.cuda.graph(graphs[1]):
-        tok = token()
+    gc.collect()        # another test's graphs must not be collected, and so destroyed, while these are captured
+    gc.disable()
+    try:
+        with torch.cuda.graph(graphs[0]):
+            outs = train()
+        with torch.cuda.graph(graphs[1]):
+            tok = token()
+    finally:
+        gc.enable()
     gen = torch.Generator().manual_seed(5)
     for _ in range(4):
         with torch.no_grad():

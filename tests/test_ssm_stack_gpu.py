@@ -213,3 +213,29 @@ def test_scorer_on_the_stack(tg):
     real, synth = rng.random((40, 24, 5)).astype(np.float32), rng.random((40, 24, 5)).astype(np.float32)
     assert 0.0 <= tg.scorer.discriminative_score(real, synth, DEV, hidden=8, steps=3, batch=16, rnn_cls=tg.SSM) <= 0.5
     assert tg.scorer.predictive_score(real, synth, DEV, hidden=8, steps=3, batch=16, rnn_cls=tg.SSM) >= 0.0
+
+
+def test_a_dropped_trainer_is_not_collected_during_a_capture(tg, monkeypatch):
+    """The graphs of a trainer that nobody holds any more go before the next capture begins, not inside it."""
+    import gc
+    import weakref
+    cfg = tg.make_cfg(features=5, hidden=8, layers=1, seq_len=24, batch_size=4)
+    x = torch.rand(4, 24, 5, device=DEV)
+
+    def trained():
+        tr = tg.TimeGANTrainer(cfg, use_graphs=True)
+        for _ in range(3):
+            tr.embedding_step(x)
+        return tr
+
+    gc.disable()
+    try:
+        gone = weakref.ref(trained())
+        assert gone() is not None, "the trainer is a cycle: only the collector frees it"
+    finally:
+        gc.enable()
+    state = []
+    real = torch.cuda.graph.__enter__
+    monkeypatch.setattr(torch.cuda.graph, "__enter__", lambda self: (state.append((gone() is None, gc.isenabled())), real(self))[1])
+    trained()
+    assert state == [(True, False)] and gc.isenabled()

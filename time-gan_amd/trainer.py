@@ -5,6 +5,7 @@ optional data parallelism (one process per GPU, gradients summed over ranks with
 A "step" here is the body of the reference's `for idx, real_data in enumerate(dl)` loop for one
 batch; the plotting / wandb block of the joint phase (TimeGANv1.py:814-896) is not part of it.
 """
+import gc
 from typing import Dict, List, Optional, Sequence
 
 from contextlib import contextmanager
@@ -43,8 +44,18 @@ class _GraphedStep:
             self.static_in = list(tensors)      # the caller's buffers become the graph's inputs
             torch.cuda.synchronize()
             self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph, capture_error_mode=self.capture_mode):
-                self.static_out = self.fn(*self.static_in)
+            # A trainer that was dropped is a reference cycle (its graphed steps hold its bound methods).  Were it
+            # collected while this capture runs, its graphs would be destroyed inside it, which ends the process: the
+            # cycles go now, and none is collected until the capture is over.
+            gc.collect()
+            collecting = gc.isenabled()
+            gc.disable()
+            try:
+                with torch.cuda.graph(self.graph, capture_error_mode=self.capture_mode):
+                    self.static_out = self.fn(*self.static_in)
+            finally:
+                if collecting:
+                    gc.enable()
         for s, t in zip(self.static_in, tensors):
             if s is not t:
                 s.copy_(t)
