@@ -121,6 +121,36 @@ def test_step_refusals(tg):
             tg.selective_scan_step(**{**kw, **change})
 
 
+def test_step_inputs_that_lie_in_the_state(tg):
+    """What a call reads beside the state must not be what it writes."""
+    pool = torch.zeros(2, 3, 4)
+    with pytest.raises(RuntimeError, match="input overlaps the state"):
+        tg.short_conv_step(pool[:, 0], pool, torch.zeros(4, 4))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tg.short_conv_step(pool[:, 0], pool, torch.zeros(4, 4), state_out=torch.zeros(2, 3, 4))
+    s = {k: v[:, 0] if v.dim() > 2 else v for k, v in scan_inputs().items()}
+    state = torch.zeros(2, 4, 16)
+    for k, v in (("u", state[..., 0].as_strided((2, 4), (64, 1))), ("delta", state.view(2, 64)[:, 8:12]), ("z", state.view(2, 64)[:, 60:]),
+                 ("B", state[:, :1]), ("C", state[:, 3:])):
+        with pytest.raises(RuntimeError, match="overlaps the state"):
+            tg.selective_scan_step(**{**s, "state": state, k: v})
+    whole = torch.zeros(2 * 64 + 8)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):      # next to it is not in it
+        tg.selective_scan_step(**{**s, "state": whole[:128].view(2, 4, 16), "u": whole[128:].view(2, 4)})
+
+
+def test_slots_and_lengths_of_other_integer_types(tg):
+    from timegan_amd import ssm
+    cpu = torch.device("cpu")
+    got = ssm._slots(torch.tensor([0, 5, -1, 2 ** 32, 2 ** 32 + 1, -2 ** 40, 2 ** 31 - 1]), cpu)
+    assert got.dtype == torch.int32 and got.tolist() == [0, 5, -1, 2 ** 31 - 1, 2 ** 31 - 1, -1, 2 ** 31 - 1]
+    assert ssm._slots([3, -1], cpu).tolist() == [3, -1]
+    assert ssm._slots(torch.tensor([200, 7], dtype=torch.uint8), cpu).tolist() == [200, 7]
+    for bad in ([0.5, 1.0], torch.tensor([True, False])):
+        with pytest.raises(RuntimeError, match="whole numbers"):
+            ssm._slots(bad, cpu)
+
+
 def test_c_abi_refuses_before_it_launches(tg):
     from timegan_amd._lib import ConvArgs, ConvStepArgs, ScanArgs, ScanStepArgs
     lb = tg.lib()
@@ -159,6 +189,11 @@ def test_size_queries(tg):
     assert lb.tgru_scan_workspace_bytes(1, 4096, 64, 16, 1, 0) > 0
     assert lb.tgru_scan_workspace_bytes(1, 4096, 64, 16, 1, 1) > lb.tgru_scan_workspace_bytes(1, 4096, 64, 16, 1, 0)
     assert lb.tgru_conv_backward_workspace_bytes(2, 24, 48, 4) >= 2 * 5 * 48 * 4
+
+
+def test_sizes_whose_state_needs_more_than_31_bits_are_refused(tg):
+    assert tg.lib().tgru_scan_workspace_bytes(1, 16, 1 << 25, 64, 1, 1) == 0
+    assert tg.lib().tgru_scan_workspace_bytes(1, 16, 1 << 24, 64, 1, 1) > 0
 
 
 def test_argument_structs_match_the_header(tg, tmp_path):

@@ -189,6 +189,33 @@ def test_offsets_beyond_32_bits(tg):
         assert torch.equal(a, b)
 
 
+def test_steps_that_lie_far_apart(tg):
+    """Steps 2^26 elements apart and more: copied in front of the scan, and the results too where they would lie like that."""
+    B, T, D, step = 2, 3, 8, 1 << 26
+    c = case_scan(10, B, T, D, 16, 1, torch.bfloat16)
+    big = torch.empty(T, step, dtype=torch.bfloat16, device=DEV)
+    far = lambda i, *shape: big.as_strided(shape, (64, step, 16, 1)[:len(shape) - 1] + (1,), 1024 * i)  # noqa: E731
+    views = {k: far(i, *c[k].shape) for i, k in enumerate(("u", "delta", "Bm", "Cm", "z", "dy"))}
+    for k, v in views.items():
+        assert v.stride(1) >= step
+        v.copy_(c[k])
+    leaves = [(views[k] if k in views else cuda(c[k])).detach().requires_grad_(True) for k in ORDER]
+    y, h = tg.selective_scan(*leaves, initial_state=cuda(c["initial"]), return_state=True)
+    grads = torch.autograd.grad([y, h], leaves, [views["dy"], cuda(c["dfinal"])])
+    dense = [cuda(c[k]).requires_grad_(True) for k in ORDER]
+    want, state = tg.selective_scan(*dense, initial_state=cuda(c["initial"]), return_state=True)
+    assert torch.equal(y, want) and torch.equal(h, state)
+    for a, b in zip(grads, torch.autograd.grad([want, state], dense, [cuda(c["dy"]), cuda(c["dfinal"])])):
+        assert torch.equal(a, b)
+    # (T, B, D) with so many sequences that a step of the result in that order would be too long
+    B, T, D = 1 << 16, 2, 1024
+    u = torch.randn(T, B, D, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+    A, b = -torch.ones(D, 4, device=DEV), torch.ones(1, 1, 1, 4, dtype=torch.bfloat16, device=DEV).expand(B, T, 1, 4)
+    y = tg.selective_scan(u, u, A, b, b)
+    few = u[-3:].contiguous()
+    assert torch.equal(y[-3:], tg.selective_scan(few, few, A, b[-3:], b[-3:]))
+
+
 # ---- convolution -----------------------------------------------------------------------------------------------------
 
 def case_conv(seed, B, T, D, K, dtype, bias=True, initial=True, lengths=None):
@@ -414,6 +441,15 @@ def test_only_what_is_asked_for(tg):
     with pytest.raises(RuntimeError, match="second derivative"):
         u = leaf(c["u"])
         torch.autograd.grad(tg.selective_scan(u, *[cuda(c[k]) for k in ORDER[1:]]).sum(), u, create_graph=True)
+
+
+def test_slots_of_64_bits(tg):
+    """A slot that 32 bits do not hold is padding like every other one outside the pool."""
+    pool = torch.randn(3, 3, 8, device=DEV)
+    was, x, w = pool.clone(), torch.randn(3, 8, device=DEV), torch.randn(8, 4, device=DEV)
+    y = tg.short_conv_step(x, pool, w, slots=torch.tensor([2 ** 32, 1, -2 ** 32], device=DEV))
+    assert not y[0].any() and not y[2].any() and y[1].any()
+    assert torch.equal(pool[0], was[0]) and torch.equal(pool[2], was[2]) and torch.equal(pool[1, -1], x[1])
 
 
 def test_steps_refuse_gradients(tg):

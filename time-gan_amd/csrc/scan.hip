@@ -902,7 +902,8 @@ int scan_dims(int B, int T, int D, int N, int G) {
     // the widest launches' workgroup numbers, and their waves', in 31 bits
     const Plan p = make_plan(B, T, D, N, G, false);
     if ((double)B * 128 * G * p.wpg * kWaves >= 2147483648.0 || (double)B * D * p.NP / 64 >= 2147483647.0 ||
-        (double)B * T * G * 2 * p.NP / 256 + (double)D * (N + 2) / 64 >= 2147483646.0 || (double)T * p.NP >= 2147483648.0)
+        (double)B * T * G * 2 * p.NP / 256 + (double)D * (N + 2) / 64 >= 2147483646.0 || (double)T * p.NP >= 2147483648.0 ||
+        (double)D * p.NP >= 2147483648.0)
         return TGRU_E_DIMS;
     return TGRU_OK;
 }

@@ -75,10 +75,13 @@ void require_gpu(const Tensor &t) {
 // Consecutive elements in the last dimension (the other strides are passed on as they are).
 Tensor rows(const Tensor &t) { return (t.size(-1) == 1 || t.stride(-1) == 1) ? t : t.contiguous(); }
 Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
+// For the scan also steps that are less than TGRU_SCAN_MAX_ROW_STRIDE elements apart.
+Tensor near_rows(const Tensor &t) { return t.stride(1) < TGRU_SCAN_MAX_ROW_STRIDE ? rows(t) : t.clone(at::MemoryFormat::Contiguous); }
 
-// A new tensor of the (B, T, D) shape of `t`, in the order of steps and sequences that `t` has in memory.
+// A new tensor of the (B, T, D) shape of `t`, in the order of steps and sequences that `t` has in memory (as far as the
+// scan's limit on the distance of two steps allows).
 Tensor like(const Tensor &t) {
-    if (t.size(0) > 1 && t.stride(1) > t.stride(0) && t.stride(0) > 0)
+    if (t.size(0) > 1 && t.stride(1) > t.stride(0) && t.stride(0) > 0 && t.size(0) * t.size(2) < TGRU_SCAN_MAX_ROW_STRIDE)
         return torch::empty({t.size(1), t.size(0), t.size(2)}, t.options()).transpose(0, 1);
     return torch::empty(t.sizes(), t.options());
 }
@@ -280,7 +283,7 @@ public:
         const auto need = ctx->saved_data["need"].toBoolList();
         const c10::hip::HIPGuardMasqueradingAsCUDA guard(in.u.device());
         tgru_scan_args a = scan_args(in, ctx->saved_data["softplus"].toBool());
-        const Tensor dy = grads[0].defined() ? rows(grads[0]) : Tensor();
+        const Tensor dy = grads[0].defined() ? near_rows(grads[0]) : Tensor();
         const Tensor dfinal = grads.size() > 1 ? dense(grads[1]) : Tensor();
         a.dy = ptr(dy);
         strides2(a.dy_stride, dy);
@@ -352,12 +355,12 @@ std::vector<Tensor> selective_scan(const Tensor &u, const Tensor &delta, const T
         require_shape(*initial_, {u.size(0), u.size(2), A.size(1)}, "initial_state");
         initial = param(*initial_, u, "initial_state");
     }
-    if (z) zz = rows(*z);
+    if (z) zz = near_rows(*z);
     require_index(lengths, u.size(0), u, "lengths");
     const Tensor A32 = param(A, u, "A");
     const OptTensor skip32 = opt_param(skip, u, "D"), bias32 = opt_param(delta_bias, u, "delta_bias");
     require_gpu(u);
-    return ScanFunction::apply(rows(u), rows(delta), A32, rows(b), rows(c), skip32, zz, bias32, initial, lengths, softplus, return_state,
+    return ScanFunction::apply(near_rows(u), near_rows(delta), A32, near_rows(b), near_rows(c), skip32, zz, bias32, initial, lengths, softplus, return_state,
                                torch::GradMode::is_enabled());
 }
 
@@ -386,6 +389,15 @@ Tensor check_pools(const Tensor &state, const OptTensor &state_out, bool slots, 
     return *state_out;
 }
 
+// An input of a one-token call lies outside the pool that the call writes.
+void apart(const Tensor &t, const Tensor &pool, const char *what) {
+    int64_t span = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) span += (t.size(i) - 1) * t.stride(i);
+    const char *p = (const char *)t.data_ptr(), *q = (const char *)pool.data_ptr();
+    TORCH_CHECK(p + span * t.element_size() <= q || q + pool.numel() * pool.element_size() <= p || !pool.numel(), what,
+                " overlaps the state that the call writes");
+}
+
 void written(const Tensor &t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -405,6 +417,7 @@ Tensor short_conv_step(const Tensor &x_, const Tensor &state, const Tensor &weig
     require_index(slots, B, x_, "slots");
     no_gradient({&x_, &state, &weight_, at(bias_), &to}, "short_conv_step");
     const Tensor x = rows(x_), weight = param(weight_, x_, "weight"), bias = bias_ ? param(*bias_, x_, "bias") : Tensor();
+    apart(x, to, "input");
     require_gpu(x_);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor y = torch::empty({B, D}, x.options());
@@ -443,6 +456,11 @@ Tensor selective_scan_step(const Tensor &u_, const Tensor &delta_, const Tensor 
     const Tensor u = rows(u_), delta = rows(delta_), b = rows(b_), c = rows(c_), z = z_ ? rows(*z_) : Tensor();
     const Tensor A32 = param(A, u, "A"), skip32 = skip ? param(*skip, u, "D") : Tensor();
     const Tensor bias32 = delta_bias ? param(*delta_bias, u, "delta_bias") : Tensor();
+    apart(u, to, "input");
+    apart(delta, to, "delta");
+    apart(b, to, "B");
+    apart(c, to, "C");
+    if (z.defined()) apart(z, to, "z");
     require_gpu(u_);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(u.device());
     Tensor y = torch::empty({B, D}, u.options());

@@ -37,7 +37,7 @@ def _lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
     if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
         if lengths.is_floating_point() or lengths.dtype == torch.bool:
             raise RuntimeError(f"lengths must be whole numbers, got {lengths.dtype}")
-        return lengths if lengths.dtype == torch.int32 else lengths.clamp(0, T).to(torch.int32)
+        return lengths if lengths.dtype == torch.int32 else lengths.long().clamp(0, T).int()
     lens = [int(v) for v in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)]
     if len(lens) != B:
         raise RuntimeError(f"Expected `len(lengths)` to be equal to batch_size, but got {len(lens)} (batch_size={B})")
@@ -51,7 +51,10 @@ def _lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
 def _slots(slots, device) -> Optional[torch.Tensor]:
     if slots is None or (isinstance(slots, torch.Tensor) and slots.dtype == torch.int32 and slots.device == device):
         return slots
-    return torch.as_tensor(slots, device=device).to(torch.int32)
+    slots = torch.as_tensor(slots, device=device)
+    if slots.is_floating_point() or slots.dtype == torch.bool:
+        raise RuntimeError(f"slots must be whole numbers, got {slots.dtype}")
+    return slots.long().clamp(-1, 2 ** 31 - 1).int()       # what 32 bits do not hold is outside every pool, and stays so
 
 
 def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *, silu: bool = True,
