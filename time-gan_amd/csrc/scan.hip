@@ -781,9 +781,12 @@ __global__ __launch_bounds__(256) void scan_grads_kernel(tgru_scan_args a, Plan 
 }
 
 // One token: a wave takes CH channels of one row.  Bound by the states, read and written once: four of them a lane, in one
-// load where N is a multiple of 4.  Rows with one slot are taken in order by the first one's wave.
-template <typename X, int S>
-__global__ __launch_bounds__(64 * kWaves) void scan_step_kernel(tgru_scan_step_args a, int tpg, int tiles, int quads) {
+// load where N is a multiple of 4.  Rows with one slot are taken in order by the first one's wave.  A wave lives for little
+// more than its chain of dependent loads, so everything whose address does not depend on the slot is requested behind the
+// slot's own load, and the states before the search for an earlier row with this slot.
+// (QUADS is a template argument because the compiler joins the two ways of loading into one, by single values, else.)
+template <typename X, int S, bool QUADS>
+__global__ __launch_bounds__(64 * kWaves) void scan_step_kernel(tgru_scan_step_args a, int tpg, int tiles) {
     constexpr int CH = 64 / S;
     const int lane = threadIdx.x & 63, c = lane / S, s = lane % S;
     const unsigned id = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -792,39 +795,55 @@ __global__ __launch_bounds__(64 * kWaves) void scan_step_kernel(tgru_scan_step_a
     const int grp = flat / tpg, Dg = a.D / a.G, first = (flat - grp * tpg) * CH;
     const bool on = c < Dg - first;
     const int d = grp * Dg + first + (on ? c : 0);
-    const int slot = a.slots ? __builtin_amdgcn_readfirstlane(a.slots[row0]) : row0;
+    const int my_slot = a.slots ? a.slots[row0] : row0;
+    __builtin_amdgcn_sched_barrier(0);
+    const int n0 = min(4 * s, QUADS ? a.N - 4 : a.N - 1);               // parts without states read the last ones
+    // four values of a row of N (zeros beyond it once they are unpacked)
+    auto four = [&](const auto *p) {
+        using E = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
+        struct alignas(4 * sizeof(E)) Pack4 { E v[4]; } q;
+        if constexpr (QUADS) {
+            q = *reinterpret_cast<const Pack4 *>(p + n0);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) q.v[k] = p[min(4 * s + k, a.N - 1)];
+        }
+        return q;
+    };
+    auto spread = [&](const auto &q, float (&v)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = 4 * s + k < a.N ? to_float(q.v[k]) : 0.f;
+    };
+    auto inputs = [&](int row) {
+        struct { decltype(four((const X *)nullptr)) b, m; X u, delta, z; } in;
+        in.u = static_cast<const X *>(a.u)[row * a.u_stride + d];
+        in.delta = static_cast<const X *>(a.delta)[row * a.delta_stride + d];
+        in.z = a.z ? static_cast<const X *>(a.z)[row * a.z_stride + d] : from_float<X>(0.f);
+        in.b = four(static_cast<const X *>(a.b) + row * a.b_stride[0] + grp * a.b_stride[1]);
+        in.m = four(static_cast<const X *>(a.c) + row * a.c_stride[0] + grp * a.c_stride[1]);
+        return in;
+    };
+    const auto rates = four(a.a + (long)d * a.N);
+    const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
+    auto in = inputs(row0);
+    __builtin_amdgcn_sched_barrier(0);
+    const int slot = __builtin_amdgcn_readfirstlane(my_slot);
     if (slot < 0 || slot >= a.P) {
         if (on && s == 0) static_cast<X *>(a.y)[row0 * a.y_stride + d] = from_float<X>(0.f);
         return;
     }
-    const int n0 = min(4 * s, quads ? a.N - 4 : a.N - 1);               // parts without states read the last ones
-    const long so = ((long)slot * a.D + d) * a.N, ao = (long)d * a.N;
-    // four values of a row of N, zeros beyond it
-    auto four = [&](const auto *p, float (&v)[4]) {
-        using E = std::remove_cv_t<std::remove_reference_t<decltype(*p)>>;
-        struct alignas(4 * sizeof(E)) Pack4 { E v[4]; };
-        if (quads) {
-            const Pack4 q = *reinterpret_cast<const Pack4 *>(p + n0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = 4 * s < a.N ? to_float(q.v[k]) : 0.f;
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = 4 * s + k < a.N ? to_float(p[min(4 * s + k, a.N - 1)]) : 0.f;
-        }
-    };
-    float h[4], a2[4];
-    four(a.state + so, h);
-    four(a.a + ao, a2);
-    const float bias = a.delta_bias ? a.delta_bias[d] : 0.f, skip = a.skip ? a.skip[d] : 0.f;
-    __builtin_amdgcn_sched_barrier(0);       // all of that is on its way while the search waits for its own loads
+    const long so = ((long)slot * a.D + d) * a.N;
+    const auto state = four(a.state + so);
+    __builtin_amdgcn_sched_barrier(0);       // on its way while the search waits for its own loads
     if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
-    for (int row = row0; row < a.B;) {
+    float h[4], a2[4];
+    spread(state, h);
+    spread(rates, a2);
+    for (int row = row0;;) {
         float b[4], m[4];
-        four(static_cast<const X *>(a.b) + row * a.b_stride[0] + grp * a.b_stride[1], b);
-        four(static_cast<const X *>(a.c) + row * a.c_stride[0] + grp * a.c_stride[1], m);
-        const float u = to_float(static_cast<const X *>(a.u)[row * a.u_stride + d]);
-        const float raw = to_float(static_cast<const X *>(a.delta)[row * a.delta_stride + d]) + bias;
-        const float z = a.z ? to_float(static_cast<const X *>(a.z)[row * a.z_stride + d]) : 0.f;
+        spread(in.b, b);
+        spread(in.m, m);
+        const float u = to_float(in.u), raw = to_float(in.delta) + bias, z = to_float(in.z);
         const float dt = a.softplus ? softplus(raw) : raw, t = dt * kLog2e;
         float y = 0.f;
 #pragma unroll
@@ -837,10 +856,12 @@ __global__ __launch_bounds__(64 * kWaves) void scan_step_kernel(tgru_scan_step_a
         if (on && s == 0) static_cast<X *>(a.y)[row * a.y_stride + d] = from_float<X>(y);
         if (!a.slots) break;
         row = find_slot(a.slots, row + 1, a.B, slot);
+        if (row >= a.B) break;
+        in = inputs(row);
     }
     if (!on || 4 * s >= a.N) return;
     float *to = a.state_out + so + 4 * s;
-    if (quads) {
+    if constexpr (QUADS) {
         *reinterpret_cast<float4 *>(to) = make_float4(h[0], h[1], h[2], h[3]);
     } else {
 #pragma unroll
@@ -1000,11 +1021,12 @@ template <typename X, int S>
 int run_scan_step(const tgru_scan_step_args &a, hipStream_t s) {
     const int CH = 64 / S, tpg = (a.D / a.G + CH - 1) / CH, tiles = tpg * a.G;
     auto ok = [](const void *p, size_t align) { return (uintptr_t)p % align == 0; };
-    const int quads = a.N % 4 == 0 && ok(a.state, 16) && ok(a.state_out, 16) && ok(a.a, 16) && ok(a.b, 4 * sizeof(X)) &&
+    const bool quads = a.N % 4 == 0 && ok(a.state, 16) && ok(a.state_out, 16) && ok(a.a, 16) && ok(a.b, 4 * sizeof(X)) &&
                       ok(a.c, 4 * sizeof(X)) && a.b_stride[0] % 4 == 0 && a.b_stride[1] % 4 == 0 && a.c_stride[0] % 4 == 0 &&
                       a.c_stride[1] % 4 == 0;
-    TGRU_LAUNCH((scan_step_kernel<X, S>), dim3((unsigned)(((long)a.B * tiles + kWaves - 1) / kWaves)), dim3(64 * kWaves), 0, s, a, tpg,
-                tiles, quads);
+    const dim3 grid((unsigned)(((long)a.B * tiles + kWaves - 1) / kWaves)), block(64 * kWaves);
+    if (quads) TGRU_LAUNCH((scan_step_kernel<X, S, true>), grid, block, 0, s, a, tpg, tiles);
+    else TGRU_LAUNCH((scan_step_kernel<X, S, false>), grid, block, 0, s, a, tpg, tiles);
     TGRU_DONE();
     return TGRU_OK;
 }

@@ -276,26 +276,29 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
     const int cv = (blockIdx.x - row0 * nblk) * 64 + (int)threadIdx.x;
     const bool on = cv < nvec;
     const int d = (on ? cv : 0) * VEC;
-    const int slot = a.slots ? __builtin_amdgcn_readfirstlane(a.slots[row0]) : row0;
+    const int my_slot = a.slots ? a.slots[row0] : row0;
+    __builtin_amdgcn_sched_barrier(0);       // what does not depend on the slot is requested behind the slot's own load
+    float w[K][VEC], bias[VEC], win[K][VEC];
+    load_taps<K, VEC>(a.weight, a.bias, d, w, bias);
+    Pack<X, VEC> x = load_pack<X, VEC>(a.x, row0 * a.x_stride + d);
+    __builtin_amdgcn_sched_barrier(0);
+    const int slot = __builtin_amdgcn_readfirstlane(my_slot);
     if (slot < 0 || slot >= a.P) {
         const float zero[VEC] = {};
         if (on) store_pack<X, VEC>(a.y, row0 * a.y_stride + d, zero);
         return;
     }
-    float w[K][VEC], bias[VEC], win[K][VEC];
-    load_taps<K, VEC>(a.weight, a.bias, d, w, bias);
     const long so = (long)slot * (K - 1) * a.D + d;
     Pack<X, VEC> st[K > 1 ? K - 1 : 1];
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) st[k] = load_pack<X, VEC>(a.state, so + (long)k * a.D);
-    __builtin_amdgcn_sched_barrier(0);       // all of that is on its way while the search waits for its own loads
+    __builtin_amdgcn_sched_barrier(0);       // on its way while the search waits for its own loads
     if (a.slots && find_slot(a.slots, 0, row0, slot) < row0) return;
 #pragma unroll
     for (int k = 0; k < K - 1; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) win[k][i] = to_float(st[k].v[i]);
-    for (int row = row0; row < a.B;) {
-        const Pack<X, VEC> x = load_pack<X, VEC>(a.x, row * a.x_stride + d);
+    for (int row = row0;;) {
         float y[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
@@ -310,6 +313,8 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
         if (on) store_pack<X, VEC>(a.y, row * a.y_stride + d, y);
         if (!a.slots) break;
         row = find_slot(a.slots, row + 1, a.B, slot);
+        if (row >= a.B) break;
+        x = load_pack<X, VEC>(a.x, row * a.x_stride + d);
     }
     if (!on) return;
 #pragma unroll

@@ -50,6 +50,7 @@ __device__ __forceinline__ int find_slot(const int32_t *__restrict__ slots, int 
         int v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = slots[min(base + 64 * k + lane, to - 1)];
+        asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));      // (else each is loaded when its turn comes)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const unsigned long long hit = __ballot(base + 64 * k + lane < to && v[k] == slot);
