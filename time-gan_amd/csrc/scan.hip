@@ -146,9 +146,12 @@ template <typename X, int S>
 struct Maps {
     static constexpr int F = Q * S, V = F < 64 ? 1 : F / 64;           // quads in all, per lane
     struct alignas(4 * sizeof(X)) Quad { X v[4]; };
+    // A quad as it is in registers: words, since two ways of loading the same four values are joined by the compiler into
+    // the slower one.
+    typedef unsigned Words __attribute__((ext_vector_type(sizeof(X)), may_alias));
     const char *base;
     long row;
-    Quad q[V];
+    Words q[V];
     __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int g) {
         base = reinterpret_cast<const char *>(static_cast<const X *>(p) + b * stride[0] + g * stride[2]);
         row = stride[1] * (long)sizeof(X);
@@ -162,10 +165,12 @@ struct Maps {
         for (int j = 0; j < V; ++j) {
             const char *r = p + (unsigned)min(first + j * (64 / S), rows) * (unsigned)row;
             if (quads) {
-                q[j] = *reinterpret_cast<const Quad *>(r + min(4 * (lane % S), N - 4) * (unsigned)sizeof(X));
+                q[j] = *reinterpret_cast<const Words *>(r + min(4 * (lane % S), N - 4) * (unsigned)sizeof(X));
             } else {
+                Quad one;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) q[j].v[k] = *reinterpret_cast<const X *>(r + min(4 * (lane % S) + k, N - 1) * (unsigned)sizeof(X));
+                for (int k = 0; k < 4; ++k) one.v[k] = *reinterpret_cast<const X *>(r + min(4 * (lane % S) + k, N - 1) * (unsigned)sizeof(X));
+                q[j] = __builtin_bit_cast(Words, one);
             }
         }
     }
@@ -174,8 +179,9 @@ struct Maps {
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int t = lane / S + j * (64 / S), n = 4 * (lane % S);
+            const Quad one = __builtin_bit_cast(Quad, q[j]);
             float4 f;
-            f.x = to_float(q[j].v[0]); f.y = to_float(q[j].v[1]); f.z = to_float(q[j].v[2]); f.w = to_float(q[j].v[3]);
+            f.x = to_float(one.v[0]); f.y = to_float(one.v[1]); f.z = to_float(one.v[2]); f.w = to_float(one.v[3]);
             if (left < Q || N < 4 * S) {
                 f.x = (t < left && n < N) ? f.x : 0.f;
                 f.y = (t < left && n + 1 < N) ? f.y : 0.f;
