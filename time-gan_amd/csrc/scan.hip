@@ -104,10 +104,20 @@ __device__ __forceinline__ void set_time(Wave &w, const Plan &pl, int T, const i
     w.tv = min(w.t_hi, clamped_length(lengths, w.b, T));
 }
 
-// Rows of a tensor of one block, split over the lanes.  All addresses are a base that is the same for the whole wave (and
-// moves by whole blocks) plus a 32-bit byte offset of the lane, so a load costs no vector arithmetic; row strides are below
-// 2^26 elements for that (kMaxRowStride).  Only a block in which the sequence ends has to hold every lane back from the
-// rows behind the end.
+// Rows of a tensor of one block, split over the lanes.  A whole block is read and written by buffer instructions: their
+// address is a base that is the same for the wave (it moves by whole blocks), a scalar offset for the row and a 32-bit byte
+// offset of the lane, so it costs no vector arithmetic (row strides are below 2^26 elements for that, kMaxRowStride), and
+// the compiler cannot join them with the loads of a block in which the sequence ends, which hold every lane back from the
+// rows behind the end.  (Joined, all of them form 64-bit addresses per lane, a tenth of the forward kernel's instructions.)
+using Block = __amdgpu_buffer_rsrc_t;
+__device__ __forceinline__ Block block_at(const char *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, -1, 0x00020000);
+}
+template <typename X>
+__device__ __forceinline__ X load_elem(Block at, unsigned lane_off, long row_off) {
+    if constexpr (sizeof(X) == 2) return __builtin_bit_cast(X, __builtin_amdgcn_raw_buffer_load_b16(at, (int)lane_off, (int)row_off, 0));
+    else return __builtin_bit_cast(X, __builtin_amdgcn_raw_buffer_load_b32(at, (int)lane_off, (int)row_off, 0));
+}
 
 // A (B, T, D) tensor: element j of a lane is step lane / CH + j S of the block, channel lane % CH of the wave.
 template <typename X, int S>
@@ -127,16 +137,23 @@ struct Rows {
     __device__ __forceinline__ void load(X (&v)[E], int t0, int left) const {
         const char *p = base + t0 * row;
         if (left >= Q) {
+            const Block at = block_at(p);
 #pragma unroll
-            for (int j = 0; j < E; ++j, p += S * row) v[j] = *reinterpret_cast<const X *>(p + lane_off);
+            for (int j = 0; j < E; ++j) v[j] = load_elem<X>(at, lane_off, j * S * row);
         } else {
 #pragma unroll
             for (int j = 0; j < E; ++j)
                 v[j] = *reinterpret_cast<const X *>(p + ((unsigned)min((int)(threadIdx.x & 63) / CH + j * S, left - 1) * (unsigned)row + col));
         }
     }
+    // element j of a block; `whole`: a block and a wave without anything missing
+    template <bool whole>
     __device__ __forceinline__ void store(int t0, int j, float v) const {
-        *reinterpret_cast<X *>(const_cast<char *>(base) + (t0 + j * S) * row + lane_off) = from_float<X>(v);
+        const X x = from_float<X>(v);
+        if constexpr (!whole) *reinterpret_cast<X *>(const_cast<char *>(base) + (t0 + j * S) * row + lane_off) = x;
+        else if constexpr (sizeof(X) == 2)
+            __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, x), block_at(base + t0 * row), (int)lane_off, (int)(j * S * row), 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), block_at(base + t0 * row), (int)lane_off, (int)(j * S * row), 0);
     }
 };
 
@@ -151,15 +168,29 @@ struct Maps {
     typedef unsigned Words __attribute__((ext_vector_type(sizeof(X)), may_alias));
     const char *base;
     long row;
+    unsigned lane_off;
     Words q[V];
-    __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int g) {
+    __device__ __forceinline__ void init(const void *p, const int64_t *stride, int b, int g, int N) {
+        const int lane = threadIdx.x & 63;
         base = reinterpret_cast<const char *>(static_cast<const X *>(p) + b * stride[0] + g * stride[2]);
         row = stride[1] * (long)sizeof(X);
+        lane_off = (unsigned)min(lane / S, Q - 1) * (unsigned)row + (unsigned)max(min(4 * (lane % S), N - 4), 0) * (unsigned)sizeof(X);
     }
     // quads: every row starts on a quad and N is a multiple of 4 -- one load instead of four
     __device__ __forceinline__ void load(int t0, int left, int N, int quads) {
         const int lane = threadIdx.x & 63;
         const char *p = base + t0 * row;
+        if (quads && left >= Q) {
+            const Block at = block_at(p);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if constexpr (sizeof(X) == 2)
+                    q[j] = __builtin_bit_cast(Words, __builtin_amdgcn_raw_buffer_load_b64(at, (int)lane_off, (int)(j * (64 / S) * row), 0));
+                else
+                    q[j] = __builtin_bit_cast(Words, __builtin_amdgcn_raw_buffer_load_b128(at, (int)lane_off, (int)(j * (64 / S) * row), 0));
+            }
+            return;
+        }
         const int first = lane / S, rows = min(left, Q) - 1;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -278,10 +309,10 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
     Maps<X, S> mb, mc;
     pu.init(a.u, a.u_stride, w.b, w.d0, w.nch);
     pd.init(a.delta, a.delta_stride, w.b, w.d0, w.nch);
-    mb.init(a.b, a.b_stride, w.b, w.g);
+    mb.init(a.b, a.b_stride, w.b, w.g, a.N);
     if (MODE == 0) {
         py.init(a.y, a.y_stride, w.b, w.d0, w.nch);
-        mc.init(a.c, a.c_stride, w.b, w.g);
+        mc.init(a.c, a.c_stride, w.b, w.g, a.N);
         if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, w.nch);
     }
     X ru[E], rd[E], rz[E];
@@ -361,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
 #pragma unroll
                     for (int q = 0; q < S; ++q) y += s_y[et][ec * S + q];
                     if (a.z) y *= z[j] * sigmoid(z[j]);
-                    py.store(t0, j, y);
+                    py.template store<decltype(full)::value>(t0, j, y);
                 }
             };
             if (full) finish(std::true_type{});
@@ -399,7 +430,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a
     Rows<X, S> pd, pz, pg;
     Maps<X, S> mc;
     pd.init(a.delta, a.delta_stride, w.b, w.d0, w.nch);
-    mc.init(a.c, a.c_stride, w.b, w.g);
+    mc.init(a.c, a.c_stride, w.b, w.g, a.N);
     if (a.dy) pg.init(a.dy, a.dy_stride, w.b, w.d0, w.nch);
     if (a.z) pz.init(a.z, a.z_stride, w.b, w.d0, w.nch);
     X rd[E], rz[E], rg[E];
@@ -532,8 +563,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
     }
     Rows<X, S> pu, pd, pz, pg, pdu, pdd, pdz;
     Maps<X, S> mb, mc;
-    mb.init(a.b, a.b_stride, w.b, w.g);
-    mc.init(a.c, a.c_stride, w.b, w.g);
+    mb.init(a.b, a.b_stride, w.b, w.g, a.N);
+    mc.init(a.c, a.c_stride, w.b, w.g, a.N);
     pu.init(a.u, a.u_stride, w.b, w.d0, load_ch);
     pd.init(a.delta, a.delta_stride, w.b, w.d0, load_ch);
     if (a.dy) pg.init(a.dy, a.dy_stride, w.b, w.d0, load_ch);
@@ -681,16 +712,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
             each([&](int j) {
                 const float du = __builtin_fmaf(sums[j].x, dt[j], skip * dy[j]);
                 bs = __builtin_fmaf(dy[j], u[j], bs);
-                if (a.du) pdu.store(t0, j, du);
+                if (a.du) pdu.template store<decltype(full)::value>(t0, j, du);
             });
             each([&](int j) {
                 const float dd = __builtin_fmaf(sums[j].x, u[j], kLn2 * sums[j].y) * slope[j];
                 bb += dd;
-                if (a.ddelta) pdd.store(t0, j, dd);
+                if (a.ddelta) pdd.template store<decltype(full)::value>(t0, j, dd);
             });
             if (a.dz)
                 each([&](int j) {
-                    pdz.store(t0, j, out[j] * __builtin_fmaf(skip, u[j], sums[j].z) * gate[j] * __builtin_fmaf(z[j], 1.f - gate[j], 1.f));
+                    pdz.template store<decltype(full)::value>(t0, j, out[j] * __builtin_fmaf(skip, u[j], sums[j].z) * gate[j] * __builtin_fmaf(z[j], 1.f - gate[j], 1.f));
                 });
         };
         if (full) finish(std::true_type{});
