@@ -10,7 +10,8 @@
  * and these entry points are what a binding for that operator would call.
  *
  * Conventions
- *   - all tensors are fp32, dense, in device memory; the caller owns every buffer; the library
+ *   - all tensors are fp32, dense, in device memory (the state-space operators at the end of this file take 16-bit
+ *     types and strides too, and say so); the caller owns every buffer; the library
  *     never allocates, frees or keeps a pointer after return; every launch goes to `stream`;
  *     no entry point synchronises with the host.
  *   - w_ih / w_hh / b_ih / b_hh (and their gradient twins) are HOST arrays of L DEVICE pointers,
@@ -432,7 +433,8 @@ int tgru_uniform(float *out, long n, unsigned long long seed, unsigned long long
  * lengths: device int32[B] or NULL; sequence b has clamp(lengths[b], 0, T) steps, in any order of lengths, zero
  * included.  Rows behind a sequence's end are never looked at (they may hold NaN); outputs and gradients there are 0.
  * No output may overlap an input or another output, except where said.
- * Every result is the same from call to call (no atomics).  Pointers need the alignment of their element type only.
+ * Every result is the same from call to call (no atomics).  Pointers need the alignment of their element type only,
+ * `reserve` and `workspace` of the scan 16 bytes (TGRU_E_ALIGN).
  * ------------------------------------------------------------------------------------------------------------- */
 
 /*

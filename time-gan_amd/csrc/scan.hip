@@ -280,6 +280,10 @@ struct Lane {
 __device__ __forceinline__ void unpack(const float4 &f, float (&v)[4]) { v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
 
 // MODE 0: the outputs.  MODE 1: a chunk's end state from a zero start and its sum of dt, for the joining kernel.
+// Bound by the vector ALU's issue: 28 instructions a wave and step (21 in MODE 1), of which 20 (16) are the four states'
+// arithmetic; it is busy in 96 % of the cycles of the second case below, in 81 % of the first.  Measured, 16 states: 64 windows of 256 steps, 1024 channels, fp32, 91 us
+// (3.7 TB/s); one sequence of 16384 steps, 2048 channels, bf16, in 32 chunks: 147 us, MODE 1 105 us and the joining 6.
+// Taking the exponentials out of the latter (wrong results) leaves 112 + 67 us, the maps' LDS reads 147 + 106.
 template <typename X, int S, int MODE>
 __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64, M = MODE == 0 ? 2 : 1;
@@ -410,7 +414,8 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
     if (a.final_state && w.chunk == pl.nchunks - 1) me.store(a.final_state, w, a.D, a.N, h);
 }
 
-// The gradient that a chunk hands to the one before it, from zero behind its end, and its sum of dt.
+// The gradient that a chunk hands to the one before it, from zero behind its end, and its sum of dt: MODE 1 above from the
+// other end, with c dy in the place of b dt u.  60 us for 4 sequences of 2048 steps, 2048 channels, bf16.
 template <typename X, int S>
 __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
@@ -525,6 +530,14 @@ __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const flo
 //     d(dt_t) = u_t (g_t . b_t) + A . w_t          dA = sum over steps dt_t w_t
 // where dy is the gradient in front of the gate.  The four waves of a workgroup are neighbouring waves of one group, one
 // sequence and one chunk: their sums over channels are joined in LDS and one row per workgroup goes to memory.
+//
+// Bound by the vector ALU's issue as well: 101 instructions a wave and step, busy in 83 % of the cycles, two waves a SIMD
+// (the states and decays of R steps are 64 registers; with bounds for three waves it spills and takes 420 us).  Measured:
+// 64 windows of 256 steps, 1024 channels, 16 states, fp32, 275 us; what is taken out of it (wrong results) saves: the sums
+// over channels 45 us, the exponentials 27, stores and their arithmetic 28, the first half's second run 20, the sums over
+// states and softplus 12 each, the joining of the four waves 7.  R = 4 is slower (289 us), and so are sums over channels
+// exchanged through LDS (318).  With N <= 8 (S = 2) a lane has twice the work per channel and the compiler spills 30 to 55
+// registers outside the loops over steps: such a call takes about as long as one with 16 states.
 template <typename X, int S>
 __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args a, Plan pl, const float *carry, float *map_part,
                                                               float *par_part) {
@@ -818,7 +831,8 @@ __global__ __launch_bounds__(256) void scan_grads_kernel(tgru_scan_args a, Plan 
 }
 
 // One token: a wave takes CH channels of one row.  Bound by the states, read and written once: four of them a lane, in one
-// load where N is a multiple of 4.  Rows with one slot are taken in order by the first one's wave.  A wave lives for little
+// load where N is a multiple of 4 (256 rows of 4096 channels with 16 states: 37 us, 3.8 TB/s; one row of 1024: 3.3 us, a
+// chain of three loads).  Rows with one slot are taken in order by the first one's wave.  A wave lives for little
 // more than its chain of dependent loads, so everything whose address does not depend on the slot is requested behind the
 // slot's own load, and the states before the search for an earlier row with this slot.
 // (QUADS is a template argument because the compiler joins the two ways of loading into one, by single values, else.)
@@ -924,8 +938,8 @@ double pass_time(long waves, long steps, const double *cost, int most) {
 
 // Chunks of time: the number that the times measured below give the shortest pass for.  A chunk more costs the main pass
 // nothing but blocks cut short; the pass in front does more of its work again (all chunks but one), and with the joining
-// costs two launches.  Measured (16 states, us a step): one sequence more or less than a round matters most -- 1280 and
-// 2048 waves of the backward pass take the same 510 us for 1024 steps, 2560 take 797.
+// costs two launches.  Measured (16 states, us a step): one sequence more or less than a round matters most -- 14 and 16
+// sequences (1792 and 2048 waves) of the backward pass take the same 503 us for 1024 steps, 20 take 708.
 Plan make_plan(int B, int T, int D, int N, int G, bool backward) {
     Plan p;
     p.NP = padded_states(N);

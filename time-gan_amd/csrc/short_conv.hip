@@ -268,7 +268,8 @@ __global__ __launch_bounds__(1024) void conv_param_grad_kernel(const float *__re
     else if (dweight) dweight[(long)d * K + k] = v;
 }
 
-// One token: a wave takes 64 VEC channels of one row.  Of the rows with one slot the first takes them all, in order,
+// One token: a wave takes 64 VEC channels of one row (256 rows of 4096 channels in 16 bits: 7 us; one row of 1024: 2.4 us,
+// a chain of two or three loads).  Of the rows with one slot the first takes them all, in order,
 // with the state in registers between them; the others' waves find that they are not the first and leave.
 template <typename X, int K, int VEC>
 __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, int nvec, int nblk) {
