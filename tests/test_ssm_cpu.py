@@ -196,6 +196,20 @@ def test_sizes_whose_state_needs_more_than_31_bits_are_refused(tg):
     assert tg.lib().tgru_scan_workspace_bytes(1, 16, 1 << 24, 64, 1, 1) > 0
 
 
+def test_launches_of_more_than_2_to_the_32_threads_are_refused(tg):
+    from timegan_amd._lib import ConvArgs, ConvStepArgs, ScanArgs, ScanStepArgs
+    lb, E_DIMS, E_NULL = tg.lib(), -1, -2
+    scan = lambda B, D: lb.tgru_scan_forward(ctypes.byref(ScanArgs(B=B, T=1, D=D, N=16, G=1)), None)  # noqa: E731
+    assert scan(1 << 20, 1024) == E_DIMS and scan(1 << 19, 1024) == E_NULL           # 16 workgroups of 256 a sequence
+    step = lambda B, D, N: lb.tgru_scan_step(ctypes.byref(ScanStepArgs(B=B, P=B, D=D, N=N, G=1)), None)  # noqa: E731
+    assert step(1 << 20, 1024, 16) == E_DIMS and step(1 << 19, 1024, 16) == E_NULL   # 64 waves a row
+    assert step(1 << 20, 1024, 4) == E_NULL and step(1 << 22, 1024, 4) == E_DIMS
+    conv = lambda B, D: lb.tgru_conv_step(ctypes.byref(ConvStepArgs(B=B, P=B, D=D, K=4)), None)  # noqa: E731
+    assert conv(1 << 22, 1024) == E_DIMS and conv(1 << 21, 1024) == E_NULL
+    back = lambda **kw: lb.tgru_conv_backward(ctypes.byref(ConvArgs(B=1, T=1, D=1 << 25, K=4, **kw)), None)  # noqa: E731
+    assert back(dweight=16, x=16, weight=16, workspace=16) == E_DIMS and back() == E_NULL
+
+
 def test_argument_structs_match_the_header(tg, tmp_path):
     """The ctypes mirrors have the layout that a C compiler gives the header's structs."""
     import os

@@ -189,6 +189,30 @@ def test_offsets_beyond_32_bits(tg):
         assert torch.equal(a, b)
 
 
+def test_gradients_of_more_rows_and_columns_than_one_launch_has_workgroups_for(tg):
+    def grads(args):
+        leaves = [a.detach().requires_grad_(True) for a in args]
+        return torch.autograd.grad(tg.selective_scan(*leaves), leaves, leaves[0].detach())
+
+    dev = torch.Generator(device=DEV).manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=dev, device=DEV)  # noqa: E731
+    B, T, D, N = 560000, 16, 4, 16                                   # 2 B T N > 2^28
+    args = [rnd(B, T, D), rnd(B, T, D), -rnd(D, N).abs(), rnd(B, T, 1, N), rnd(B, T, 1, N), rnd(D)]
+    many = grads(args)
+    for part in (slice(0, 3), slice(B - 3, B)):
+        few = grads([a[part] if a.shape[0] == B else a for a in args])
+        for k in (0, 1, 3, 4):
+            assert torch.equal(many[k][part], few[k])
+    D = 300000                                                       # D (N + 2) > 2^22
+    args = [rnd(1, 2, D), rnd(1, 2, D), -rnd(D, N).abs(), rnd(1, 2, 1, N), rnd(1, 2, 1, N), rnd(D)]
+    many = grads(args)
+    part = slice(D - 32, D)
+    few = grads([args[0][..., part], args[1][..., part], args[2][part], args[3], args[4], args[5][part]])
+    for k in (2, 5):
+        assert torch.equal(many[k][part], few[k]) and torch.equal(many[k][:32], grads(
+            [args[0][..., :32], args[1][..., :32], args[2][:32], args[3], args[4], args[5][:32]])[k])
+
+
 def test_steps_that_lie_far_apart(tg):
     """Steps 2^26 elements apart and more: copied in front of the scan, and the results too where they would lie like that."""
     B, T, D, step = 2, 3, 8, 1 << 26

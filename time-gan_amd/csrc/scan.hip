@@ -29,6 +29,7 @@
 // second kernel joins the chunks in order, and the main pass starts every chunk from its joined state.  The backward
 // pass does the same from the other end.
 #include "ssm_common.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace tgru {
@@ -793,41 +794,46 @@ template <typename X>
 __global__ __launch_bounds__(256) void scan_grads_kernel(tgru_scan_args a, Plan pl, const float *__restrict__ map_part, unsigned map_blocks,
                                                          const float *__restrict__ par_part) {
     if (blockIdx.x < map_blocks) {
-        const long per = (long)a.T * pl.NP, id = (long)blockIdx.x * 256 + threadIdx.x;     // (b, g, db | dc, t, n)
-        const long part = id / per, bg = part >> 1;
-        const int e = (int)(id - part * per), t = e / pl.NP, n = e - t * pl.NP;
-        if (bg >= (long)a.B * a.G || n >= a.N) return;
-        const int b = (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
-        float v = 0.f;
-        if (t < clamped_length(a.lengths, b, a.T)) {
-            const float *p = map_part + (bg * pl.wpg * 2 + (part & 1)) * per + e;
+        const long per = (long)a.T * pl.NP, all = (long)a.B * a.G * 2 * per;
+        for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < all; id += (long)map_blocks * 256) {     // (b, g, db | dc, t, n)
+            const long part = id / per, bg = part >> 1;
+            const int e = (int)(id - part * per), t = e / pl.NP, n = e - t * pl.NP;
+            if (n >= a.N) continue;
+            const int b = (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
+            float v = 0.f;
+            if (t < clamped_length(a.lengths, b, a.T)) {
+                const float *p = map_part + (bg * pl.wpg * 2 + (part & 1)) * per + e;
 #pragma unroll 8
-            for (int q = 0; q < pl.wpg; ++q) v += p[q * 2 * per];
+                for (int q = 0; q < pl.wpg; ++q) v += p[q * 2 * per];
+            }
+            X *to = static_cast<X *>((part & 1) ? a.dc : a.db);
+            if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
         }
-        X *to = static_cast<X *>((part & 1) ? a.dc : a.db);
-        if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
         return;
     }
     __shared__ float red[4][64];
     const int c = threadIdx.x & 63, grp = threadIdx.x >> 6, rows = a.B * pl.nchunks;
-    const long cols = (long)a.D * (a.N + 2), col = (long)(blockIdx.x - map_blocks) * 64 + c;
     const int each = (rows + 3) / 4, r0 = grp * each, r1 = min(rows, r0 + each);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (col < cols) {
-        int r = r0;
-        for (; r + 3 < r1; r += 4)
+    const long cols = (long)a.D * (a.N + 2), dn = (long)a.D * a.N;
+    for (long col0 = (long)(blockIdx.x - map_blocks) * 64; col0 < cols; col0 += (long)(gridDim.x - map_blocks) * 64) {
+        const long col = col0 + c;
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
+        if (col < cols) {
+            int r = r0;
+            for (; r + 3 < r1; r += 4)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) s[q] += par_part[(long)(r + q) * cols + col];
-        for (; r < r1; ++r) s[0] += par_part[(long)r * cols + col];
+                for (int q = 0; q < 4; ++q) s[q] += par_part[(long)(r + q) * cols + col];
+            for (; r < r1; ++r) s[0] += par_part[(long)r * cols + col];
+        }
+        __syncthreads();
+        red[grp][c] = (s[0] + s[1]) + (s[2] + s[3]);
+        __syncthreads();
+        if (grp != 0 || col >= cols) continue;
+        const float v = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+        if (col < dn) { if (a.da) a.da[col] = v; }
+        else if (col < dn + a.D) { if (a.dskip) a.dskip[col - dn] = v; }
+        else if (a.ddelta_bias) a.ddelta_bias[col - dn - a.D] = v;
     }
-    red[grp][c] = (s[0] + s[1]) + (s[2] + s[3]);
-    __syncthreads();
-    if (grp != 0 || col >= cols) return;
-    const float v = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-    const long dn = (long)a.D * a.N;
-    if (col < dn) { if (a.da) a.da[col] = v; }
-    else if (col < dn + a.D) { if (a.dskip) a.dskip[col - dn] = v; }
-    else if (a.ddelta_bias) a.ddelta_bias[col - dn - a.D] = v;
 }
 
 // One token: a wave takes CH channels of one row.  Bound by the states, read and written once: four of them a lane, in one
@@ -971,12 +977,13 @@ Plan make_plan(int B, int T, int D, int N, int G, bool backward) {
 int scan_dims(int B, int T, int D, int N, int G) {
     if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || N > TGRU_SCAN_MAX_STATES || D % G) return TGRU_E_DIMS;
     if (T > (1 << 30) || D > (1 << 26)) return TGRU_E_DIMS;
-    // the widest launches' workgroup numbers, and their waves', in 31 bits
-    const Plan p = make_plan(B, T, D, N, G, false);
-    if ((double)B * 128 * G * p.wpg * kWaves >= 2147483648.0 || (double)B * D * p.NP / 64 >= 2147483647.0 ||
-        (double)B * T * G * 2 * p.NP / 256 + (double)D * (N + 2) / 64 >= 2147483646.0 || (double)T * p.NP >= 2147483648.0 ||
-        (double)D * p.NP >= 2147483648.0)
-        return TGRU_E_DIMS;
+    // a launch holds less than 2^32 threads, and offsets within one sequence's maps or state are 32-bit numbers
+    for (bool backward : {false, true}) {
+        const Plan p = make_plan(B, T, D, N, G, backward);
+        if ((double)B * p.nchunks * G * p.wpg * 64 * kWaves >= 4294967296.0 || (double)T * p.NP >= 2147483648.0 ||
+            (double)D * p.NP >= 2147483648.0 || (p.nchunks > 1 && (double)B * D * p.NP >= 4294967232.0))
+            return TGRU_E_DIMS;
+    }
     return TGRU_OK;
 }
 
@@ -1031,8 +1038,9 @@ int run_scan(const tgru_scan_args &a, bool backward, hipStream_t s) {
     TGRU_LAUNCH((scan_bwd_kernel<X, S>), grid, block, 0, s, a, pl, carry, map, par);
     TGRU_DONE();
     if (map || par) {
-        const unsigned maps = map ? (unsigned)(((long)a.B * a.G * a.T * 2 * pl.NP + 255) / 256) : 0;
-        const unsigned pars = par ? (unsigned)(((long)a.D * (a.N + 2) + 63) / 64) : 0;
+        // (workgroups beyond these numbers take turns)
+        const unsigned maps = map ? (unsigned)std::min<long>(((long)a.B * a.G * a.T * 2 * pl.NP + 255) / 256, 1 << 20) : 0;
+        const unsigned pars = par ? (unsigned)std::min<long>(((long)a.D * (a.N + 2) + 63) / 64, 1 << 16) : 0;
         TGRU_LAUNCH((scan_grads_kernel<X>), dim3(maps + pars), dim3(256), 0, s, a, pl, map, maps, par);
         TGRU_DONE();
     }
@@ -1118,7 +1126,10 @@ int tgru_scan_backward(const tgru_scan_args *a, tgru_stream_t stream) { return s
 int tgru_scan_step(const tgru_scan_step_args *a, tgru_stream_t stream) {
     if (!a) return TGRU_E_NULL;
     if (a->B <= 0 || a->P <= 0 || a->D <= 0 || a->N <= 0 || a->G <= 0 || a->N > TGRU_SCAN_MAX_STATES || a->D % a->G) return TGRU_E_DIMS;
-    if ((!a->slots && a->P < a->B) || (double)a->B * a->D >= 2147483648.0) return TGRU_E_DIMS;
+    if (!a->slots && a->P < a->B) return TGRU_E_DIMS;
+    // less than 2^32 threads
+    const int CH = 256 / (a->N <= 4 ? 4 : padded_states(a->N)), tpg = (a->D / a->G - 1) / CH + 1;
+    if ((double)a->B * tpg * a->G >= 67108860.0) return TGRU_E_DIMS;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     if (!a->u || !a->delta || !a->b || !a->c || !a->a || !a->state || !a->state_out || !a->y) return TGRU_E_NULL;
     if (int rc = tgru::check_device()) return rc;

@@ -451,6 +451,8 @@ int tgru_conv_backward(const tgru_conv_args *a, tgru_stream_t stream) {
     if (!a) return TGRU_E_NULL;
     if (int rc = conv_dims(a->B, a->T, a->D, a->K)) return rc;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
+    // the parameter gradients' launch holds less than 2^32 threads, 32 a column
+    if ((a->dweight || a->dbias) && (double)(a->K + 1) * a->D >= 134217696.0) return TGRU_E_DIMS;
     if (!a->x || !a->weight || ((a->dweight || a->dbias) && !a->workspace)) return TGRU_E_NULL;
     if (int rc = tgru::check_device()) return rc;
     tgru_conv_args c = *a;
@@ -461,7 +463,8 @@ int tgru_conv_backward(const tgru_conv_args *a, tgru_stream_t stream) {
 int tgru_conv_step(const tgru_conv_step_args *a, tgru_stream_t stream) {
     if (!a) return TGRU_E_NULL;
     if (a->B <= 0 || a->P <= 0 || a->D <= 0 || a->K <= 0 || a->K > TGRU_CONV_MAX_TAPS) return TGRU_E_DIMS;
-    if ((long)a->B * ((a->D + 63) / 64) >= (1L << 31) || a->D > (1 << 30) || (!a->slots && a->P < a->B)) return TGRU_E_DIMS;
+    // less than 2^32 threads
+    if (a->D > (1 << 30) || (long)a->B * ((a->D + 63) / 64) >= (1L << 26) || (!a->slots && a->P < a->B)) return TGRU_E_DIMS;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     if (!a->x || !a->weight || !a->y || (a->K > 1 && (!a->state || !a->state_out))) return TGRU_E_NULL;
     if (int rc = tgru::check_device()) return rc;
