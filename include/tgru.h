@@ -497,7 +497,7 @@ int tgru_conv_step(const tgru_conv_step_args *a, tgru_stream_t stream);
  * `workspace`: tgru_scan_workspace_bytes(..., backward) bytes.
  */
 #define TGRU_SCAN_MAX_STATES 64
-#define TGRU_SCAN_MAX_ROW_STRIDE (1 << 26) /* strides from step to step are below this many elements (TGRU_E_DIMS) */
+#define TGRU_SCAN_MAX_ROW_STRIDE (1 << 25) /* strides from step to step are below this many elements (TGRU_E_DIMS) */
 typedef struct tgru_scan_args {
     const void *u, *delta, *z, *b, *c;
     const float *a, *skip, *delta_bias;

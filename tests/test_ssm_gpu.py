@@ -189,6 +189,22 @@ def test_offsets_beyond_32_bits(tg):
         assert torch.equal(a, b)
 
 
+def test_steps_almost_too_far_apart_to_be_read_in_place(tg):
+    B, T, D, step = 1, 20, 24, (1 << 25) - 64
+    c = case_scan(11, B, T, D, 16, 1, torch.float32)
+    big = torch.empty(T, step, device=DEV)
+    views = {k: big.as_strided((B,) + tuple(c[k].shape[1:]), (0, step, 16, 1)[:c[k].dim() - 1] + (1,), 64 * i)
+             for i, k in enumerate(("u", "delta", "Bm", "Cm", "z", "dy"))}
+    for k, v in views.items():
+        v.copy_(c[k])
+    leaves = [(views[k] if k in views else cuda(c[k])).detach().requires_grad_(True) for k in ORDER]
+    dense = [cuda(c[k]).requires_grad_(True) for k in ORDER]
+    y, want = tg.selective_scan(*leaves), tg.selective_scan(*dense)
+    assert torch.equal(y, want)
+    for a, b in zip(torch.autograd.grad(y, leaves, views["dy"]), torch.autograd.grad(want, dense, cuda(c["dy"]))):
+        assert torch.equal(a, b)
+
+
 def test_gradients_of_more_rows_and_columns_than_one_launch_has_workgroups_for(tg):
     def grads(args):
         leaves = [a.detach().requires_grad_(True) for a in args]

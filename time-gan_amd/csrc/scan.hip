@@ -107,7 +107,8 @@ __device__ __forceinline__ void set_time(Wave &w, const Plan &pl, int T, const i
 
 // Rows of a tensor of one block, split over the lanes.  A whole block is read and written by buffer instructions: their
 // address is a base that is the same for the wave (it moves by whole blocks), a scalar offset for the row and a 32-bit byte
-// offset of the lane, so it costs no vector arithmetic (row strides are below 2^26 elements for that, kMaxRowStride), and
+// offset of the lane, so it costs no vector arithmetic (row strides are below 2^25 elements for that, kMaxRowStride: 15 rows
+// of 4-byte elements are offsets below 2^31), and
 // the compiler cannot join them with the loads of a block in which the sequence ends, which hold every lane back from the
 // rows behind the end.  (Joined, all of them form 64-bit addresses per lane, a tenth of the forward kernel's instructions.)
 using Block = __amdgpu_buffer_rsrc_t;
@@ -976,7 +977,7 @@ Plan make_plan(int B, int T, int D, int N, int G, bool backward) {
 
 int scan_dims(int B, int T, int D, int N, int G) {
     if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || N > TGRU_SCAN_MAX_STATES || D % G) return TGRU_E_DIMS;
-    if (T > (1 << 30) || D > (1 << 26)) return TGRU_E_DIMS;
+    if (T > (1 << 30) || D >= kMaxRowStride) return TGRU_E_DIMS;
     // a launch holds less than 2^32 threads, and offsets within one sequence's maps or state are 32-bit numbers
     for (bool backward : {false, true}) {
         const Plan p = make_plan(B, T, D, N, G, backward);
