@@ -790,47 +790,57 @@ __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args
 
 // The gradients that several workgroups of scan_bwd_kernel have a share of; everything is added in a fixed order.
 //   workgroups [0, map_blocks): db, dc (B, T, G, N) from map_part[b][g][workgroup][db, dc][t][NP]; zeros behind the end
-//   the others: da, dskip, ddelta_bias from the rows of par_part[rows][D (N + 2)], 64 columns x 4 groups of rows each
+//   the others: da, dskip, ddelta_bias from the rows of par_part[rows][D (N + 2)], 32 columns x 8 groups of rows each
 template <typename X>
 __global__ __launch_bounds__(256) void scan_grads_kernel(tgru_scan_args a, Plan pl, const float *__restrict__ map_part, unsigned map_blocks,
                                                          const float *__restrict__ par_part) {
     if (blockIdx.x < map_blocks) {
-        const long per = (long)a.T * pl.NP, all = (long)a.B * a.G * 2 * per;
-        for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < all; id += (long)map_blocks * 256) {     // (b, g, db | dc, t, n)
-            const long part = id / per, bg = part >> 1;
-            const int e = (int)(id - part * per), t = e / pl.NP, n = e - t * pl.NP;
+        // four states a thread; (b, g, db | dc, t, quad of states)
+        const int quads = pl.NP / 4, shift = __builtin_ctz(quads);
+        const long per = (long)a.T * quads, all = (long)a.B * a.G * 2 * per, stride = (long)map_blocks * 256;
+        struct alignas(sizeof(X)) Four { X v[4]; };
+        for (long id = (long)blockIdx.x * 256 + threadIdx.x; id < all; id += stride) {
+            const long part = all < 4294967296L ? (long)((unsigned)id / (unsigned)per) : id / per, bg = part >> 1;
+            const int e = (int)(id - part * per), t = e >> shift, n = (e & (quads - 1)) * 4;
             if (n >= a.N) continue;
-            const int b = (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
-            float v = 0.f;
+            const int b = a.G == 1 ? (int)bg : (int)(bg / a.G), g = (int)(bg - (long)b * a.G);
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (t < clamped_length(a.lengths, b, a.T)) {
-                const float *p = map_part + (bg * pl.wpg * 2 + (part & 1)) * per + e;
+                const float4 *p = reinterpret_cast<const float4 *>(map_part) + (bg * pl.wpg * 2 + (part & 1)) * per + e;
 #pragma unroll 8
-                for (int q = 0; q < pl.wpg; ++q) v += p[q * 2 * per];
+                for (int q = 0; q < pl.wpg; ++q) {
+                    const float4 f = p[q * 2 * per];
+                    v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+                }
             }
             X *to = static_cast<X *>((part & 1) ? a.dc : a.db);
-            if (to) to[(((long)b * a.T + t) * a.G + g) * a.N + n] = from_float<X>(v);
+            if (!to) continue;
+            to += (((long)b * a.T + t) * a.G + g) * a.N + n;
+            const Four four = {{from_float<X>(v.x), from_float<X>(v.y), from_float<X>(v.z), from_float<X>(v.w)}};
+            if (n + 4 <= a.N) {
+                *reinterpret_cast<Four *>(to) = four;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 3; ++k)
+                    if (n + k < a.N) to[k] = four.v[k];
+            }
         }
         return;
     }
-    __shared__ float red[4][64];
-    const int c = threadIdx.x & 63, grp = threadIdx.x >> 6, rows = a.B * pl.nchunks;
-    const int each = (rows + 3) / 4, r0 = grp * each, r1 = min(rows, r0 + each);
+    __shared__ float red[8][32];
+    const int c = threadIdx.x & 31, grp = threadIdx.x >> 5, rows = a.B * pl.nchunks;
+    const int each = (rows + 7) / 8, r0 = grp * each, r1 = min(rows, r0 + each);
     const long cols = (long)a.D * (a.N + 2), dn = (long)a.D * a.N;
-    for (long col0 = (long)(blockIdx.x - map_blocks) * 64; col0 < cols; col0 += (long)(gridDim.x - map_blocks) * 64) {
+    for (long col0 = (long)(blockIdx.x - map_blocks) * 32; col0 < cols; col0 += (long)(gridDim.x - map_blocks) * 32) {
         const long col = col0 + c;
-        float s[4] = {0.f, 0.f, 0.f, 0.f};
-        if (col < cols) {
-            int r = r0;
-            for (; r + 3 < r1; r += 4)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) s[q] += par_part[(long)(r + q) * cols + col];
-            for (; r < r1; ++r) s[0] += par_part[(long)r * cols + col];
-        }
+        const float s = col < cols ? sum_rows(par_part + col, cols, r0, r1) : 0.f;
         __syncthreads();
-        red[grp][c] = (s[0] + s[1]) + (s[2] + s[3]);
+        red[grp][c] = s;
         __syncthreads();
         if (grp != 0 || col >= cols) continue;
-        const float v = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v += red[q][c];
         if (col < dn) { if (a.da) a.da[col] = v; }
         else if (col < dn + a.D) { if (a.dskip) a.dskip[col - dn] = v; }
         else if (a.ddelta_bias) a.ddelta_bias[col - dn - a.D] = v;
@@ -1040,8 +1050,8 @@ int run_scan(const tgru_scan_args &a, bool backward, hipStream_t s) {
     TGRU_DONE();
     if (map || par) {
         // (workgroups beyond these numbers take turns)
-        const unsigned maps = map ? (unsigned)std::min<long>(((long)a.B * a.G * a.T * 2 * pl.NP + 255) / 256, 1 << 20) : 0;
-        const unsigned pars = par ? (unsigned)std::min<long>(((long)a.D * (a.N + 2) + 63) / 64, 1 << 16) : 0;
+        const unsigned maps = map ? (unsigned)std::min<long>(((long)a.B * a.G * a.T * pl.NP / 2 + 255) / 256, 1 << 18) : 0;
+        const unsigned pars = par ? (unsigned)std::min<long>(((long)a.D * (a.N + 2) + 31) / 32, 1 << 17) : 0;
         TGRU_LAUNCH((scan_grads_kernel<X>), dim3(maps + pars), dim3(256), 0, s, a, pl, map, maps, par);
         TGRU_DONE();
     }

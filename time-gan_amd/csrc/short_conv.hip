@@ -7,6 +7,7 @@
 // requested together; only the K - 1 rows in front of a run are read twice (out of the cache: the run before has them).
 // Lanes run over channels first, so a wave's loads are consecutive.
 #include "ssm_common.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace tgru {
@@ -15,8 +16,10 @@ namespace ssm {
 constexpr int kConvThreads = 256;
 constexpr int kRows = 8, kRowsBack = 2;      // rows requested together
 
+// Neighbouring channels of a row, loaded and stored by one instruction wherever they start (the chip takes wide accesses at
+// any element's alignment).
 template <typename X, int VEC>
-struct alignas(sizeof(X) * VEC) Pack { X v[VEC]; };
+struct alignas(sizeof(X)) Pack { X v[VEC]; };
 
 template <typename X, int VEC>
 __device__ __forceinline__ Pack<X, VEC> load_pack(const void *base, long elem) {
@@ -30,7 +33,9 @@ __device__ __forceinline__ void store_pack(void *base, long elem, const float (&
     *reinterpret_cast<Pack<X, VEC> *>(static_cast<X *>(base) + elem) = p;
 }
 
-// Where a thread stands: channels [d, d + VEC) of sequence b, steps [t0, t1) of its n, run number `row` of all runs.
+// Where a thread stands: channels [d, d + VEC) of sequence b, steps [t0, t1) of its n, run number `row` of all runs.  The
+// last pack of a row ends with the row: where VEC does not divide D, it and the pack before it both compute, and write,
+// what they share.
 struct Place { int b, d, t0, t1, n, run; long row; bool live; };
 
 template <int VEC>
@@ -39,7 +44,7 @@ __device__ __forceinline__ Place place_of(const tgru_conv_args &a, int nvec, int
     const unsigned id = blockIdx.x * kConvThreads + threadIdx.x;
     const unsigned r = id / (unsigned)nvec;
     p.live = r < (unsigned)a.B * (unsigned)runs;
-    p.d = (int)(id - r * (unsigned)nvec) * VEC;
+    p.d = min((int)(id - r * (unsigned)nvec) * VEC, a.D - VEC);
     p.b = (int)(r / (unsigned)runs);
     p.run = (int)(r - (unsigned)p.b * (unsigned)runs);
     p.row = r;
@@ -62,7 +67,7 @@ __device__ __forceinline__ void input_row(const tgru_conv_args &a, const Place &
     for (int i = 0; i < VEC; ++i) v[i] = to_float(r.v[i]);
 }
 
-// The taps of VEC channels lie next to each other; with packs they start on 16 bytes.
+// The taps of VEC channels lie next to each other.
 template <int K, int VEC>
 __device__ __forceinline__ void load_taps(const float *weight, const float *bias, int d, float (&w)[K][VEC], float (&b)[VEC]) {
     float flat[K * VEC];
@@ -70,8 +75,9 @@ __device__ __forceinline__ void load_taps(const float *weight, const float *bias
     if constexpr (VEC >= 4) {
 #pragma unroll
         for (int j = 0; j < K * VEC / 4; ++j) {
-            const float4 v = reinterpret_cast<const float4 *>(from)[j];
-            flat[4 * j] = v.x; flat[4 * j + 1] = v.y; flat[4 * j + 2] = v.z; flat[4 * j + 3] = v.w;
+            const Pack<float, 4> four = reinterpret_cast<const Pack<float, 4> *>(from)[j];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) flat[4 * j + i] = four.v[i];
         }
     } else {
 #pragma unroll
@@ -241,28 +247,29 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(tgru_conv_args a
     for (int i = 0; i < VEC; ++i) part[(long)K * a.D + i] = db[i];
 }
 
-// dweight (D, K) and dbias (D) from the rows part[rows][K + 1][D]: 32 columns x 32 groups of rows per workgroup, a
-// group adds a contiguous range, the groups are joined in order.
-__global__ __launch_bounds__(1024) void conv_param_grad_kernel(const float *__restrict__ part, int rows, int D, int K,
-                                                               float *dweight, float *dbias) {
+// Sums of the rows part[rows][K + 1][D]: 32 columns x 32 groups of rows per workgroup, a group adds a contiguous range, the
+// groups are joined in order.  FOLD: workgroup row y of the launch leaves the sums of rows [y, y + 1) * kFold in row y of
+// `folded`; otherwise they are dweight (D, K) and dbias (D).  Many rows of few columns are folded first, because a column
+// block is one workgroup: 16384 rows of 240 columns take 9.5 us, 36 in one launch.
+constexpr int kFold = 512;
+template <bool FOLD>
+__global__ __launch_bounds__(1024) void conv_param_grad_kernel(const float *__restrict__ part, int rows, int D, int K, float *dweight, float *dbias,
+                                                               float *folded) {
     __shared__ float red[32][33];
     const int c = threadIdx.x & 31, grp = threadIdx.x >> 5;
     const long cols = (long)(K + 1) * D, col = (long)blockIdx.x * 32 + c;
-    const int per = (rows + 31) / 32, r0 = grp * per, r1 = min(rows, r0 + per);
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (col < cols) {
-        int r = r0;
-        for (; r + 3 < r1; r += 4)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) s[q] += part[(long)(r + q) * cols + col];
-        for (; r < r1; ++r) s[0] += part[(long)r * cols + col];
-    }
-    red[grp][c] = (s[0] + s[1]) + (s[2] + s[3]);
+    const int first = FOLD ? (int)blockIdx.y * kFold : 0, end = FOLD ? min(rows, first + kFold) : rows;
+    const int per = (end - first + 31) / 32, r0 = min(end, first + grp * per), r1 = min(end, r0 + per);
+    red[grp][c] = col < cols ? sum_rows(part + col, cols, r0, r1) : 0.f;
     __syncthreads();
     if (grp != 0 || col >= cols) return;
     float v = 0.f;
 #pragma unroll
     for (int q = 0; q < 32; ++q) v += red[q][c];
+    if (FOLD) {
+        folded[blockIdx.y * cols + col] = v;
+        return;
+    }
     const int k = (int)(col / D), d = (int)(col - (long)k * D);
     if (k == K) { if (dbias) dbias[d] = v; }
     else if (dweight) dweight[(long)d * K + k] = v;
@@ -322,37 +329,32 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
     for (int k = 0; k < K - 1; ++k) store_pack<X, VEC>(a.state_out, so + (long)k * a.D, win[k]);
 }
 
-// Steps per run: as long as the launch still has about `waves` waves, because the K - 1 rows around a run are read
-// twice; 8 at least (one group of loads), 64 at most.  16-byte packs need few waves to fill the memory's queues, single
-// elements many.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 48 us with 2048 waves (5.5 TB/s), 58 with 4096, 71
-// with 8192; backward 95 us with 2048 (4.2 TB/s).  7 x 1531 steps of 1003 channels, single elements: 12 us with 8192, 16
-// with 2048.
+// Steps per run: as long as the launch still has about `waves` waves, because the K - 1 rows around a run are read twice; 8 at
+// least (one group of loads), 64 at most.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 48 us with 2048
+// waves (5.5 TB/s), 58 with 4096, 71 with 8192; backward 95 us with 2048 (4.2 TB/s).
 int conv_run_len(int B, int T, int nvec, long waves) {
     int len = 64;
     while (len > 8 && (long)B * ((T + len - 1) / len) * nvec < waves * 64) len >>= 1;
     return len;
 }
-constexpr long kConvWaves = 2048, kConvWavesSingle = 8192;
+constexpr long kConvWaves = 2048;
 
-bool multiple_of(long v, long m) { return v % m == 0; }
-
-// 16-byte packs where every row of every tensor of the call starts on one, single elements otherwise.
-bool conv_packs(const tgru_conv_args &a, bool backward) {
-    const int vec = 16 / (int)dtype_bytes(a.dtype);
-    auto ok = [&](const void *p, const int64_t *st) {
-        return !p || (((uintptr_t)p & 15) == 0 && (!st || (multiple_of(st[0], vec) && multiple_of(st[1], vec))));
-    };
-    bool v = a.D % vec == 0 && ok(a.weight, nullptr) && ok(a.x, a.x_stride) && ok(a.initial_state, nullptr);
-    if (!backward) return v && ok(a.y, a.y_stride) && ok(a.final_state, nullptr);
-    return v && ok(a.dy, a.dy_stride) && ok(a.dx, a.dx_stride) && ok(a.dfinal, nullptr) && ok(a.dinitial, nullptr);
+// Packs of 16 bytes wherever a row has as many channels, single elements otherwise.  (8 x 4096 steps of 2003 channels in 16 bits
+// with single elements, forward 59 us, with packs 51; 64 x 256 steps of 1021: 20 and 17.)
+int conv_vec(int D, int dtype) {
+    const int vec = 16 / (int)dtype_bytes(dtype);
+    return D >= vec ? vec : 1;
 }
+
+// Whether the rows of partial sums are folded first: more than four round trips a thread otherwise, and columns for less than
+// half of the chip.  Measured, in one launch / folded: 2048 rows of 240 columns 6.2 / 7.7 us, 3072 rows of 960 columns 8.8 / 7.6.
+bool conv_folds(long rows, long cols) { return rows > 4 * kFold && cols < 128 * 32; }
 
 template <typename X, int K>
 int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
-    const bool packs = conv_packs(a, backward);
-    const int vec = packs ? 16 / (int)sizeof(X) : 1;
-    const int nvec = a.D / vec;
-    const int len = conv_run_len(a.B, a.T, nvec, packs || backward ? kConvWaves : kConvWavesSingle), runs = (a.T + len - 1) / len;
+    const int vec = conv_vec(a.D, a.dtype), nvec = (a.D + vec - 1) / vec;
+    const bool packs = vec > 1;
+    const int len = conv_run_len(a.B, a.T, nvec, kConvWaves), runs = (a.T + len - 1) / len;
     const dim3 grid((unsigned)(((long)a.B * runs * nvec + kConvThreads - 1) / kConvThreads)), block(kConvThreads);
     constexpr int VEC = 16 / (int)sizeof(X);
     if (!backward) {
@@ -365,8 +367,18 @@ int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
     if (hipGetLastError() != hipSuccess) return TGRU_E_LAUNCH;
     if (a.dweight || a.dbias) {
         const long cols = (long)(K + 1) * a.D;
-        TGRU_LAUNCH(conv_param_grad_kernel, dim3((unsigned)((cols + 31) / 32)), dim3(1024), 0, s, a.workspace, a.B * runs,
-                    a.D, K, a.dweight, a.dbias);
+        const unsigned blocks = (unsigned)((cols + 31) / 32);
+        const float *part = a.workspace;
+        int rows = a.B * runs;
+        if (conv_folds(rows, cols)) {
+            const int folds = (rows + kFold - 1) / kFold;
+            float *folded = a.workspace + rows * cols;
+            TGRU_LAUNCH(conv_param_grad_kernel<true>, dim3(blocks, (unsigned)folds), dim3(1024), 0, s, part, rows, a.D, K, nullptr, nullptr, folded);
+            if (hipGetLastError() != hipSuccess) return TGRU_E_LAUNCH;
+            part = folded;
+            rows = folds;
+        }
+        TGRU_LAUNCH(conv_param_grad_kernel<false>, dim3(blocks), dim3(1024), 0, s, part, rows, a.D, K, a.dweight, a.dbias, nullptr);
     }
     return hipGetLastError() == hipSuccess ? TGRU_OK : TGRU_E_LAUNCH;
 }
@@ -374,9 +386,7 @@ int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
 template <typename X, int K>
 int run_conv_step(const tgru_conv_step_args &a, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(X);
-    auto ok = [](const void *p) { return ((uintptr_t)p & 15) == 0; };
-    const bool packs = a.D % VEC == 0 && ok(a.weight) && ok(a.x) && ok(a.y) && ok(a.state) && ok(a.state_out) &&
-                       multiple_of(a.x_stride, VEC) && multiple_of(a.y_stride, VEC);
+    const bool packs = a.D % VEC == 0;       // (no shared channels here: the state may be updated where it lies)
     const int nvec = packs ? a.D / VEC : a.D, nblk = (nvec + 63) / 64;
     const dim3 grid((unsigned)((long)a.B * nblk)), block(64);
     if (packs) TGRU_LAUNCH((conv_step_kernel<X, K, VEC>), grid, block, 0, s, a, nvec, nblk);
@@ -424,15 +434,13 @@ extern "C" {
 
 size_t tgru_conv_backward_workspace_bytes(int B, int T, int D, int K) {
     if (conv_dims(B, T, D, K) != TGRU_OK) return 0;
-    // the packs' run length is not known here (it goes by pointers and strides): room for the shortest runs of the
-    // widest and of the narrowest packs
+    // the element type is not known here: room for the shorter runs of the two sizes of packs
     size_t rows = 0;
-    for (int vec = 1; vec <= 8; vec *= 2) {
-        if (D % vec) break;
-        const int len = conv_run_len(B, T, D / vec, kConvWaves);
-        const size_t r = (size_t)B * ((T + len - 1) / len);
-        if (r > rows) rows = r;
+    for (int dtype : {TGRU_DTYPE_F32, TGRU_DTYPE_BF16}) {
+        const int vec = conv_vec(D, dtype), len = conv_run_len(B, T, (D + vec - 1) / vec, kConvWaves);
+        rows = std::max(rows, (size_t)B * ((T + len - 1) / len));
     }
+    if (conv_folds((long)rows, (long)(K + 1) * D)) rows += (rows + kFold - 1) / kFold;
     return rows * (size_t)(K + 1) * D * sizeof(float);
 }
 
