@@ -315,6 +315,29 @@ def test_conv_lengths_and_what_lies_behind_them(tg, D, dtype):
     assert not got[0].cpu()[~on].any() and not got[2]["x"].cpu()[~on].any()
 
 
+@pytest.mark.parametrize("B,T,D,K,dtype", [(3000, 9, 3, 4, torch.float32), (700, 40, 13, 3, torch.bfloat16), (2100, 5, 9, 1, torch.float16),
+                                           (5000, 3, 17, 8, torch.float32)])
+def test_conv_parameter_gradients_over_many_sequences(tg, B, T, D, K, dtype):
+    """More rows of partial sums than are added in one launch."""
+    g = torch.Generator().manual_seed(B)
+    c = case_conv(B, B, T, D, K, dtype, lengths=torch.randint(0, T + 1, (B,), generator=g).tolist())
+    check_conv(c, run_conv(tg, c, True), True)
+
+
+def test_conv_gradients_of_millions_of_sequences(tg):
+    """Two million rows, against sums in 64 bits.  A term is rounded once and goes through two rounds of at most 128 rows of a
+    thread, 16 partial sums and 32 threads: less than 384 roundings of 2^-24 each."""
+    B, D, K = 2200000, 2, 2
+    dev = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = (torch.randn(B, 1, D, generator=dev, device=DEV) for _ in range(2))
+    w, b = torch.randn(D, K, generator=dev, device=DEV).requires_grad_(True), torch.zeros(D, device=DEV, requires_grad=True)
+    dw, db = torch.autograd.grad(tg.short_conv(x, w, b, silu=False), (w, b), dy)
+    want, size = (dy.double() * x.double()).sum((0, 1)), (dy.double() * x.double()).abs().sum((0, 1))
+    eps = 384 * 2.0 ** -24
+    assert ((dw[:, -1].double() - want).abs() <= eps * size).all() and not dw[:, 0].any()
+    assert ((db.double() - dy.double().sum((0, 1))).abs() <= eps * dy.double().abs().sum((0, 1))).all()
+
+
 def test_conv_strides_and_alignment(tg):
     c = case_conv(6, 3, 50, 32, 4, torch.bfloat16)
     plain = run_conv(tg, c, True)

@@ -248,17 +248,17 @@ __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(tgru_conv_args a
 }
 
 // Sums of the rows part[rows][K + 1][D]: 32 columns x 32 groups of rows per workgroup, a group adds a contiguous range, the
-// groups are joined in order.  FOLD: workgroup row y of the launch leaves the sums of rows [y, y + 1) * kFold in row y of
+// groups are joined in order.  FOLD: workgroup row y of the launch leaves the sums of rows [y, y + 1) * fold in row y of
 // `folded`; otherwise they are dweight (D, K) and dbias (D).  Many rows of few columns are folded first, because a column
 // block is one workgroup: 16384 rows of 240 columns take 9.5 us, 36 in one launch.
-constexpr int kFold = 512;
+constexpr int kFold = 512, kMaxFolds = 4096;
 template <bool FOLD>
 __global__ __launch_bounds__(1024) void conv_param_grad_kernel(const float *__restrict__ part, int rows, int D, int K, float *dweight, float *dbias,
-                                                               float *folded) {
+                                                               float *folded, int fold) {
     __shared__ float red[32][33];
     const int c = threadIdx.x & 31, grp = threadIdx.x >> 5;
     const long cols = (long)(K + 1) * D, col = (long)blockIdx.x * 32 + c;
-    const int first = FOLD ? (int)blockIdx.y * kFold : 0, end = FOLD ? min(rows, first + kFold) : rows;
+    const int first = FOLD ? (int)blockIdx.y * fold : 0, end = FOLD ? min(rows - first, fold) + first : rows;
     const int per = (end - first + 31) / 32, r0 = min(end, first + grp * per), r1 = min(end, r0 + per);
     red[grp][c] = col < cols ? sum_rows(part + col, cols, r0, r1) : 0.f;
     __syncthreads();
@@ -349,6 +349,7 @@ int conv_vec(int D, int dtype) {
 // Whether the rows of partial sums are folded first: more than four round trips a thread otherwise, and columns for less than
 // half of the chip.  Measured, in one launch / folded: 2048 rows of 240 columns 6.2 / 7.7 us, 3072 rows of 960 columns 8.8 / 7.6.
 bool conv_folds(long rows, long cols) { return rows > 4 * kFold && cols < 128 * 32; }
+int conv_fold(long rows) { return (int)std::max<long>(kFold, (rows + kMaxFolds - 1) / kMaxFolds); }
 
 template <typename X, int K>
 int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
@@ -371,14 +372,16 @@ int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
         const float *part = a.workspace;
         int rows = a.B * runs;
         if (conv_folds(rows, cols)) {
-            const int folds = (rows + kFold - 1) / kFold;
+            const int fold = conv_fold(rows), folds = (rows + fold - 1) / fold;
             float *folded = a.workspace + rows * cols;
-            TGRU_LAUNCH(conv_param_grad_kernel<true>, dim3(blocks, (unsigned)folds), dim3(1024), 0, s, part, rows, a.D, K, nullptr, nullptr, folded);
+            TGRU_LAUNCH(conv_param_grad_kernel<true>, dim3(blocks, (unsigned)folds), dim3(1024), 0, s, part, rows, a.D, K, nullptr, nullptr, folded,
+                        fold);
             if (hipGetLastError() != hipSuccess) return TGRU_E_LAUNCH;
             part = folded;
             rows = folds;
         }
-        TGRU_LAUNCH(conv_param_grad_kernel<false>, dim3(blocks), dim3(1024), 0, s, part, rows, a.D, K, a.dweight, a.dbias, nullptr);
+        TGRU_LAUNCH(conv_param_grad_kernel<false>, dim3(blocks), dim3(1024), 0, s, part, rows, a.D, K, a.dweight, a.dbias, nullptr,
+                    0);
     }
     return hipGetLastError() == hipSuccess ? TGRU_OK : TGRU_E_LAUNCH;
 }
@@ -440,7 +443,7 @@ size_t tgru_conv_backward_workspace_bytes(int B, int T, int D, int K) {
         const int vec = conv_vec(D, dtype), len = conv_run_len(B, T, (D + vec - 1) / vec, kConvWaves);
         rows = std::max(rows, (size_t)B * ((T + len - 1) / len));
     }
-    if (conv_folds((long)rows, (long)(K + 1) * D)) rows += (rows + kFold - 1) / kFold;
+    if (conv_folds((long)rows, (long)(K + 1) * D)) rows += std::min<size_t>((rows + kFold - 1) / kFold, kMaxFolds);
     return rows * (size_t)(K + 1) * D * sizeof(float);
 }
 
