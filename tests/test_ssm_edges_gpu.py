@@ -1,0 +1,43 @@
+"""The state-space operators at the edges of their arguments' ranges, on the GPU: states that grow, rates that are infinite,
+results that are changed in place, views and large sizes.  Values against ssm_reference.py (float64), with its bounds."""
+import pytest
+import torch
+
+import ssm_reference as ref
+from test_ssm_gpu import DEV, ORDER, case_scan, check_scan, cuda, randn, run_scan, tg  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def growing_scan(tg, N):  # noqa: F811
+    """300 steps of few channels: cut into chunks of 16 or 32 steps (checked).  A step of -0.5 multiplies a state by up to
+    e^8, so a chunk of such steps by up to 2^369, far beyond float32."""
+    c = case_scan(21, 1, 300, 24, N, 1, torch.float32, bias=False)
+    c["A"] = -16 * (0.5 + 0.5 * torch.rand(24, N, generator=torch.Generator().manual_seed(1)))
+    assert tg.lib().tgru_scan_workspace_bytes(1, 300, 24, N, 1, 0) > 0
+    return c
+
+
+@pytest.mark.parametrize("N", [16, 5])
+def test_a_state_of_zero_stays_zero_where_states_grow(tg, N):  # noqa: F811
+    """Nothing enters before the last 8 steps and no gradient behind the first 8: in between all is 0, whatever the chunks
+    would make of a state.  8 steps are e^64 at most, and the exponents' errors of 12 half steps times 64 are within
+    ref.bound's 8 T = 2400."""
+    c = growing_scan(tg, N)
+    c["delta"] = torch.full_like(c["delta"], -0.5)
+    c["u"][:, :-8] = 0
+    c["dy"][:, 8:] = 0
+    c["initial"], c["dfinal"] = torch.zeros_like(c["initial"]), torch.zeros_like(c["dfinal"])
+    check_scan(c, run_scan(tg, c, softplus=False), softplus=False)
+
+
+@pytest.mark.parametrize("N", [16, 5])
+def test_a_small_state_grows_by_more_than_float_holds(tg, N):  # noqa: F811
+    """13 steps in one chunk multiply by up to e^104 = 2^150, what enters is about 1e-30: 1e15 comes out, in both directions.
+    12 * 104 half steps from the exponents are within ref.bound."""
+    c = growing_scan(tg, N)
+    c["delta"] = torch.zeros_like(c["delta"])
+    c["delta"][:, 97:110] = -0.5
+    for k in ("initial", "dfinal", "u", "dy"):
+        c[k] = c[k] * 1e-30
+    check_scan(c, run_scan(tg, c, softplus=False), softplus=False)

@@ -493,6 +493,15 @@ __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a
     if (me.s == 0) sdt[((long)w.b * pl.nchunks + w.chunk) * a.D + w.d0 + me.c] = dts;
 }
 
+// 2^x h + v.  The growth of a whole chunk may be beyond float (negative steps, positive rates: 32 steps of half a unit at a
+// rate of 16 are 2^185) where what it makes of a small state, or of none, is not, so the whole part of x goes into the exponent
+// of h: 0 stays 0, and the rest is a factor in [1, 2).  (Beyond 4000 every float but 0 has left the range; a NaN that this
+// loses is in v as well.)
+__device__ __forceinline__ float add_grown(float h, float x, float v) {
+    const float in = fminf(fmaxf(x, -4000.f), 4000.f), whole = floorf(in);
+    return __builtin_fmaf(__builtin_amdgcn_ldexpf(h, (int)whole), __builtin_amdgcn_exp2f(in - whole), v);
+}
+
 // Joins the chunks: carry[chunk] becomes what enters the chunk.  (What the last one in the order of the pass would hand on
 // was not computed: its slot is read, and what comes of it is not used.)  `edge`: (B, D, N) entering the first chunk in the
 // order of the pass (the initial state forward, the final state's gradient backward), or null.  One thread per state.
@@ -520,8 +529,7 @@ __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const flo
             if (i0 + r >= pl.nchunks) break;
             state[(backward ? pl.nchunks - 1 - (i0 + r) : i0 + r) * per] = h;
             // a chunk without steps passes the state on as it is, also where A is infinite
-            const float p = dt[r] == 0.f ? 1.f : __builtin_amdgcn_exp2f(dt[r] * a2);
-            h = __builtin_fmaf(p, h, v[r]);
+            h = add_grown(h, dt[r] == 0.f ? 0.f : dt[r] * a2, v[r]);
         }
     }
 }
