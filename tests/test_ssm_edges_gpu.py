@@ -41,3 +41,24 @@ def test_a_small_state_grows_by_more_than_float_holds(tg, N):  # noqa: F811
     for k in ("initial", "dfinal", "u", "dy"):
         c[k] = c[k] * 1e-30
     check_scan(c, run_scan(tg, c, softplus=False), softplus=False)
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("N", [16, 5])
+def test_a_token_with_infinite_rates(tg, N, softplus):  # noqa: F811
+    """A = -inf forgets the state at every step that is longer than 0; one of length 0 (also softplus of -200) keeps it.  The
+    same from a sequence of one step and from the one-token form."""
+    c = case_scan(23, 4, 1, 8, N, 1, torch.float32, bias=False)
+    c["A"] = torch.full_like(c["A"], float("-inf"))
+    zero = -200.0 if softplus else 0.0
+    c["delta"] = torch.tensor([0.5, zero, 1.0, zero])[:, None, None].expand(4, 1, 8).contiguous()
+    s = {k: cuda(c[k]) for k in ORDER}
+    y_seq, h_seq = tg.selective_scan(*[s[k] for k in ORDER], softplus=softplus, initial_state=cuda(c["initial"]), return_state=True)
+    state = cuda(c["initial"]).clone()
+    y = tg.selective_scan_step(s["u"][:, 0], s["delta"][:, 0], state, s["A"], s["Bm"][:, 0], s["Cm"][:, 0], s["D"], s["z"][:, 0],
+                               softplus=softplus)
+    c["A"] = torch.full_like(c["A"], -1e30)
+    args = [c[k] for k in ORDER]
+    want, size = (ref.scan(*args, softplus=softplus, initial=c["initial"], absolute=a) for a in (False, True))
+    for got, k, what in ((y_seq, 0, "sequence"), (h_seq, 1, "its state"), (y[:, None], 0, "token"), (state, 1, "its state")):
+        ref.close(got, want[k], size[k], 1, what=what)

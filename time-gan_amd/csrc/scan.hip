@@ -246,9 +246,12 @@ __device__ __forceinline__ bool place_wave(Wave &w, const tgru_scan_args &a, con
     return true;
 }
 
+// An infinite rate is taken as 3e38: the same decay to nothing for every dt > 0, and a step of dt = 0 leaves the state as it
+// is (0 times infinity would not).
+__device__ __forceinline__ float finite_rate(float v) { return __builtin_isinf(v) ? __builtin_copysignf(3.0e38f, v) : v; }
+
 // This lane's four states: where they are in a row of carry or ckpt, and their rates to base 2 per unit of dt.  Steps behind
-// a sequence's end are staged as dt = 0, which leaves a state as it is, exactly: exp2(0 a2) = 1 for every finite a2 (an
-// infinite one is taken as 3e38: the same decay to nothing for every dt > 0).
+// a sequence's end are staged as dt = 0, which leaves a state as it is, exactly: exp2(0 a2) = 1 for every finite a2.
 template <int S>
 struct Lane {
     int c, s;                        // channel of the wave, part of the channel
@@ -262,8 +265,7 @@ struct Lane {
         at = (long)(w.d0 + (on ? c : 0)) * (4 * S) + 4 * s;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const float v = has(k, N) ? rates[(long)(w.d0 + c) * N + 4 * s + k] * kLog2e : 0.f;
-            a2[k] = __builtin_isinf(v) ? __builtin_copysignf(3.0e38f, v) : v;
+            a2[k] = has(k, N) ? finite_rate(rates[(long)(w.d0 + c) * N + 4 * s + k] * kLog2e) : 0.f;
         }
     }
     __device__ __forceinline__ bool has(int k, int N) const { return on && 4 * s + k < N; }
@@ -915,6 +917,8 @@ __global__ __launch_bounds__(64 * kWaves) void scan_step_kernel(tgru_scan_step_a
     float h[4], a2[4];
     spread(state, h);
     spread(rates, a2);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) a2[k] = finite_rate(a2[k]);
     for (int row = row0;;) {
         float b[4], m[4];
         spread(in.b, b);
