@@ -366,10 +366,14 @@ std::vector<Tensor> selective_scan(const Tensor &u, const Tensor &delta, const T
 
 // ---- one token -------------------------------------------------------------------------------------------------------
 
+// Neither direction of automatic differentiation passes through a one-token call.  (Tangents of forward mode are there under
+// torch.no_grad() too.)
 void no_gradient(std::initializer_list<const Tensor *> ts, const char *what) {
-    if (!torch::GradMode::is_enabled()) return;
-    for (const Tensor *t : ts)
-        TORCH_CHECK(!(t && t->defined() && t->requires_grad()), what, " has no backward pass: call it under torch.no_grad()");
+    for (const Tensor *t : ts) {
+        if (!t || !t->defined()) continue;
+        TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative: its inputs must not be dual tensors");
+        TORCH_CHECK(!(torch::GradMode::is_enabled() && t->requires_grad()), what, " has no backward pass: call it under torch.no_grad()");
+    }
 }
 
 const Tensor *at(const OptTensor &t) { return t ? &*t : nullptr; }
