@@ -62,3 +62,24 @@ def test_a_token_with_infinite_rates(tg, N, softplus):  # noqa: F811
     want, size = (ref.scan(*args, softplus=softplus, initial=c["initial"], absolute=a) for a in (False, True))
     for got, k, what in ((y_seq, 0, "sequence"), (h_seq, 1, "its state"), (y[:, None], 0, "token"), (state, 1, "its state")):
         ref.close(got, want[k], size[k], 1, what=what)
+
+
+def test_results_in_order_of_time_can_be_changed_in_place(tg):  # noqa: F811
+    """(T, B, D) inputs give results in that order; they are tensors of their own, not views that autograd protects."""
+    g = torch.Generator().manual_seed(1)
+    x, w, s = randn(g, 6, 3, 16).to(DEV), randn(g, 16, 4).to(DEV), randn(g, 16).to(DEV)
+    A, b = -torch.ones(16, 4, device=DEV), randn(g, 3, 6, 1, 4).to(DEV)
+    calls = (lambda t: tg.short_conv(t, w), lambda t: tg.short_conv(t, w, return_state=True)[0],
+             lambda t: tg.selective_scan(t, t, A, b, b), lambda t: tg.selective_scan(t, t, A, b, b, return_state=True)[0])
+    for call in calls:
+        leaf = x.clone().requires_grad_(True)
+        want = torch.autograd.grad((call(leaf.transpose(0, 1)) * s).sum(), leaf)[0]
+        y = call(leaf.transpose(0, 1))
+        assert y.stride() == (16, 48, 1) and not y._is_view()
+        y.mul_(s)
+        assert torch.equal(torch.autograd.grad(y.sum(), leaf)[0], want)
+        scale = s.clone().requires_grad_(True)        # a result without a graph, changed by something with one
+        y = call(x.transpose(0, 1))
+        before = y.clone()
+        y.mul_(scale)
+        assert torch.equal(torch.autograd.grad(y.sum(), scale)[0], before.sum((0, 1)))

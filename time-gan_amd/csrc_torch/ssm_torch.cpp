@@ -79,10 +79,10 @@ Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 Tensor near_rows(const Tensor &t) { return t.stride(1) < TGRU_SCAN_MAX_ROW_STRIDE ? rows(t) : t.clone(at::MemoryFormat::Contiguous); }
 
 // A new tensor of the (B, T, D) shape of `t`, in the order of steps and sequences that `t` has in memory (as far as the
-// scan's limit on the distance of two steps allows).
+// scan's limit on the distance of two steps allows).  Not a view: autograd forbids to change a view that a function returns.
 Tensor like(const Tensor &t) {
     if (t.size(0) > 1 && t.stride(1) > t.stride(0) && t.stride(0) > 0 && t.size(0) * t.size(2) < TGRU_SCAN_MAX_ROW_STRIDE)
-        return torch::empty({t.size(1), t.size(0), t.size(2)}, t.options()).transpose(0, 1);
+        return torch::empty_strided(t.sizes(), {t.size(2), t.size(0) * t.size(2), 1}, t.options());
     return torch::empty(t.sizes(), t.options());
 }
 
