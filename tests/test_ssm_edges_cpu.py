@@ -20,3 +20,13 @@ def test_steps_refuse_dual_tensors(tg, grad):  # noqa: F811
                     fn(**{**args, k: dual})
             with pytest.raises(RuntimeError, match="no CPU fallback"):
                 fn(**args)
+
+
+def test_slots_out_of_a_table(tg):  # noqa: F811
+    """A column of an int32 table is taken like any other whole numbers."""
+    table = torch.tensor([[6, 0], [2, 1], [3, 2]], dtype=torch.int32)
+    scan = {k: v[:, 0] if v.dim() > 2 else v for k, v in scan_inputs(B=3).items()}
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tg.short_conv_step(torch.zeros(3, 4), torch.zeros(8, 3, 4), torch.zeros(4, 4), slots=table[:, 0])
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        tg.selective_scan_step(**scan, state=torch.zeros(8, 4, 16), slots=table[:, 0])

@@ -83,3 +83,14 @@ def test_results_in_order_of_time_can_be_changed_in_place(tg):  # noqa: F811
         before = y.clone()
         y.mul_(scale)
         assert torch.equal(torch.autograd.grad(y.sum(), scale)[0], before.sum((0, 1)))
+
+
+def test_lengths_and_slots_out_of_a_table(tg):  # noqa: F811
+    """Columns of an int32 table on the GPU, whose elements are not consecutive."""
+    g = torch.Generator().manual_seed(2)
+    x, w, pool = randn(g, 3, 6, 8).to(DEV), randn(g, 8, 4).to(DEV), randn(g, 8, 3, 8).to(DEV)
+    table = torch.tensor([[6, 5], [2, 0], [3, 1]], dtype=torch.int32, device=DEV)
+    assert torch.equal(tg.short_conv(x, w, lengths=table[:, 0]), tg.short_conv(x, w, lengths=[6, 2, 3]))
+    first, second = pool.clone(), pool.clone()
+    assert torch.equal(tg.short_conv_step(x[:, 0], first, w, slots=table[:, 1]), tg.short_conv_step(x[:, 0], second, w, slots=[5, 0, 1]))
+    assert torch.equal(first, second)

@@ -37,7 +37,7 @@ def _lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
     if isinstance(lengths, torch.Tensor) and lengths.is_cuda:
         if lengths.is_floating_point() or lengths.dtype == torch.bool:
             raise RuntimeError(f"lengths must be whole numbers, got {lengths.dtype}")
-        return lengths if lengths.dtype == torch.int32 else lengths.long().clamp(0, T).int()
+        return lengths.contiguous() if lengths.dtype == torch.int32 else lengths.long().clamp(0, T).int()
     lens = [int(v) for v in (lengths.tolist() if isinstance(lengths, torch.Tensor) else lengths)]
     if len(lens) != B:
         raise RuntimeError(f"Expected `len(lengths)` to be equal to batch_size, but got {len(lens)} (batch_size={B})")
@@ -49,8 +49,10 @@ def _lengths(lengths, B: int, T: int, device) -> Optional[torch.Tensor]:
 
 
 def _slots(slots, device) -> Optional[torch.Tensor]:
-    if slots is None or (isinstance(slots, torch.Tensor) and slots.dtype == torch.int32 and slots.device == device):
-        return slots
+    if slots is None:
+        return None
+    if isinstance(slots, torch.Tensor) and slots.dtype == torch.int32 and slots.device == device:
+        return slots.contiguous()
     slots = torch.as_tensor(slots, device=device)
     if slots.is_floating_point() or slots.dtype == torch.bool:
         raise RuntimeError(f"slots must be whole numbers, got {slots.dtype}")
@@ -81,7 +83,7 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     state (P, K - 1, D) in x's type, dense, is a pool of states; row i of x belongs to state[slots[i]] (state[i] without
     slots).  The states are updated in place, or written to state_out (same shape) with `state` left as it was.  A row
     whose slot is outside [0, P) is padding: y is 0, no state is touched.  Rows with the same slot are steps of one sequence
-    and are taken in order.  slots: int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
+    and are taken in order.  slots: dense int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
     not overlap the states that are written (refused).  No backward pass.
     """
     return _op().short_conv_step(x, state, weight, bias, silu, _slots(slots, x.device), state_out)
