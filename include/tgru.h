@@ -432,8 +432,9 @@ int tgru_uniform(float *out, long n, unsigned long long seed, unsigned long long
  * gradients and scan states are fp32 and dense.  All arithmetic is fp32; outputs are rounded once.
  * lengths: device int32[B] or NULL; sequence b has clamp(lengths[b], 0, T) steps, in any order of lengths, zero
  * included.  Rows behind a sequence's end are never looked at (they may hold NaN); outputs and gradients there are 0.
- * No output may overlap an input or another output, except where said.  Sizes that one launch cannot hold (2^32 threads) are
- * refused (TGRU_E_DIMS).
+ * No output may overlap an input or another output, except where said.  Sizes that one launch cannot hold (2^32 threads: for
+ * the convolution one for up to 64 steps of 16 bytes of channels; for its one-token form B ceil(D / 64) < 2^26) are refused
+ * (TGRU_E_DIMS), and so are scans of 2^31 values or more of T steps' or D channels' states (each rounded up to 8, 16, 32 or 64).
  * Every result is the same from call to call (no atomics).  Pointers need the alignment of their element type only,
  * `reserve` and `workspace` of the scan 16 bytes (TGRU_E_ALIGN).
  * ------------------------------------------------------------------------------------------------------------- */

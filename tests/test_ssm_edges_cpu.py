@@ -30,3 +30,19 @@ def test_slots_out_of_a_table(tg):  # noqa: F811
         tg.short_conv_step(torch.zeros(3, 4), torch.zeros(8, 3, 4), torch.zeros(4, 4), slots=table[:, 0])
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         tg.selective_scan_step(**scan, state=torch.zeros(8, 4, 16), slots=table[:, 0])
+
+
+def test_convolutions_that_one_launch_holds_are_taken(tg):  # noqa: F811
+    """The launch has a thread for 64 steps of 16 bytes of channels, so 2^35 elements are far from 2^32 threads."""
+    import ctypes
+    from timegan_amd._lib import ConvArgs
+    lb, E_DIMS, E_NULL = tg.lib(), -1, -2
+    for dims, want in (((32, 131072, 8192), E_NULL), ((520, 4096, 8192), E_NULL), ((1 << 20, 4096, 64), E_NULL), ((1 << 27, 1, 64), E_NULL),
+                       ((1, 8, (1 << 31) - 256), E_NULL), ((1, 8, (1 << 31) - 255), E_DIMS), ((1, 1, (1 << 31) - 1), E_DIMS),
+                       ((1 << 30, 128, 1), E_DIMS), ((1 << 29, 64, 64), E_DIMS), ((1 << 28, 64, 256), E_DIMS)):
+        for dtype in (0, 1, 2):
+            args = ctypes.byref(ConvArgs(**dict(zip("BTD", dims)), K=4, dtype=dtype))
+            assert lb.tgru_conv_forward(args, None) == want and lb.tgru_conv_backward(args, None) == want, (dims, dtype)
+        assert (lb.tgru_conv_backward_workspace_bytes(*dims, 4) > 0) == (want == E_NULL)
+    for dtype, want in ((0, E_DIMS), (1, E_NULL), (2, E_NULL)):       # 2^32 and 2^31 packs of one step
+        assert lb.tgru_conv_forward(ctypes.byref(ConvArgs(B=1 << 26, T=1, D=256, K=4, dtype=dtype)), None) == want

@@ -94,3 +94,30 @@ def test_lengths_and_slots_out_of_a_table(tg):  # noqa: F811
     first, second = pool.clone(), pool.clone()
     assert torch.equal(tg.short_conv_step(x[:, 0], first, w, slots=table[:, 1]), tg.short_conv_step(x[:, 0], second, w, slots=[5, 0, 1]))
     assert torch.equal(first, second)
+
+
+def test_a_convolution_of_more_than_2_to_the_34_elements(tg):  # noqa: F811
+    """520 sequences, all the same one (so inputs are small), results whole: 35 GB each.  Without the activation a term of
+    dweight is an exact product; it goes through 64 steps of a run, at most 80 rows of partial sums in a thread and its
+    tree, and 32 threads: less than 256 roundings."""
+    B, T, D, K = 520, 4096, 8192, 4
+    dev = torch.Generator(device=DEV).manual_seed(4)
+    rnd = lambda *s: torch.randn(*s, generator=dev, device=DEV)  # noqa: E731
+    one, dy, w = rnd(1, T, D).bfloat16(), rnd(1, T, D).bfloat16(), rnd(D, K)
+    assert B * T * D > 2 ** 34
+    results = []
+    for n in (1, B):
+        x = one.expand(n, T, D).detach().requires_grad_(True)
+        weight = w.clone().requires_grad_(True)
+        y = tg.short_conv(x, weight, silu=False)
+        results.append((y.detach(), *torch.autograd.grad(y, [x, weight], dy.expand(n, T, D))))
+        del y
+    (y1, dx1, _), (y, dx, dw) = results
+    for i in (0, 255, 256, B - 1):
+        assert torch.equal(y[i], y1[0]) and torch.equal(dx[i], dx1[0])
+    ext = torch.cat([one.new_zeros(1, K - 1, D), one], 1)[0].double()
+    for k in range(K):
+        terms = dy[0].double() * ext[k:k + T]
+        assert ((dw[:, k].double() - B * terms.sum(0)).abs() <= 256 * 2.0 ** -24 * B * terms.abs().sum(0)).all()
+    del results, y, dx
+    torch.cuda.empty_cache()

@@ -421,11 +421,13 @@ int dispatch_conv_step(const tgru_conv_step_args &a, hipStream_t s) {
 #undef TGRU_CALL
 }
 
-// B * T rows and their D channels have to fit the launch's 32-bit thread numbers with single elements and runs of 8.
-int conv_dims(int B, int T, int D, int K) {
+// A launch has a thread for every run and pack, numbered in 32 bits, and the runs (rows of partial sums) are counted in 31.
+int conv_dims(int B, int T, int D, int K, int dtype) {
     if (B <= 0 || T <= 0 || D <= 0 || K <= 0 || K > TGRU_CONV_MAX_TAPS) return TGRU_E_DIMS;
-    if (T > (1 << 30) || (double)B * ((T + 7) / 8) * D > 2147483648.0 - kConvThreads) return TGRU_E_DIMS;
-    return TGRU_OK;
+    if (T > (1 << 30) || D > INT32_MAX - kConvThreads + 1) return TGRU_E_DIMS;
+    const int vec = conv_vec(D, dtype), nvec = (D + vec - 1) / vec, len = conv_run_len(B, T, nvec, kConvWaves);
+    const double runs = (double)B * ((T + len - 1) / len);
+    return runs < 2147483648.0 && runs * nvec < 4294967296.0 - kConvThreads ? TGRU_OK : TGRU_E_DIMS;
 }
 
 }  // namespace ssm
@@ -436,20 +438,21 @@ using namespace tgru::ssm;
 extern "C" {
 
 size_t tgru_conv_backward_workspace_bytes(int B, int T, int D, int K) {
-    if (conv_dims(B, T, D, K) != TGRU_OK) return 0;
     // the element type is not known here: room for the shorter runs of the two sizes of packs
     size_t rows = 0;
     for (int dtype : {TGRU_DTYPE_F32, TGRU_DTYPE_BF16}) {
+        if (conv_dims(B, T, D, K, dtype) != TGRU_OK) continue;
         const int vec = conv_vec(D, dtype), len = conv_run_len(B, T, (D + vec - 1) / vec, kConvWaves);
         rows = std::max(rows, (size_t)B * ((T + len - 1) / len));
     }
+    if (!rows) return 0;
     if (conv_folds((long)rows, (long)(K + 1) * D)) rows += std::min<size_t>((rows + kFold - 1) / kFold, kMaxFolds);
     return rows * (size_t)(K + 1) * D * sizeof(float);
 }
 
 int tgru_conv_forward(const tgru_conv_args *a, tgru_stream_t stream) {
     if (!a) return TGRU_E_NULL;
-    if (int rc = conv_dims(a->B, a->T, a->D, a->K)) return rc;
+    if (int rc = conv_dims(a->B, a->T, a->D, a->K, a->dtype)) return rc;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     if (!a->x || !a->weight || !a->y) return TGRU_E_NULL;
     if (int rc = tgru::check_device()) return rc;
@@ -460,7 +463,7 @@ int tgru_conv_forward(const tgru_conv_args *a, tgru_stream_t stream) {
 
 int tgru_conv_backward(const tgru_conv_args *a, tgru_stream_t stream) {
     if (!a) return TGRU_E_NULL;
-    if (int rc = conv_dims(a->B, a->T, a->D, a->K)) return rc;
+    if (int rc = conv_dims(a->B, a->T, a->D, a->K, a->dtype)) return rc;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     // the parameter gradients' launch holds less than 2^32 threads, 32 a column
     if ((a->dweight || a->dbias) && (double)(a->K + 1) * a->D >= 134217696.0) return TGRU_E_DIMS;
