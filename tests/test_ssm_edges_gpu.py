@@ -121,3 +121,13 @@ def test_a_convolution_of_more_than_2_to_the_34_elements(tg):  # noqa: F811
         assert ((dw[:, k].double() - B * terms.sum(0)).abs() <= 256 * 2.0 ** -24 * B * terms.abs().sum(0)).all()
     del results, y, dx
     torch.cuda.empty_cache()
+
+
+def test_accuracy_of_the_activation(tg):  # noqa: F811
+    """v sigmoid(v) through a convolution of one tap of 1, relative to the value.  Half steps of float32: exp2 and the reciprocal
+    2 each, the sum, the product and the result 1 each; below 0 also |v| for the rounded exponent v log2(e) and 0.22 |v| for the
+    constant's own rounding (2^-26.2)."""
+    v = torch.linspace(-80, 80, 1 << 20)
+    y = tg.short_conv(v.view(-1, 1, 1).to(DEV), torch.ones(1, 1, device=DEV)).cpu().view(-1).double()
+    want = v.double() * torch.sigmoid(v.double())
+    assert ((y - want).abs() <= (7 - 1.22 * v.double().clamp(max=0)) * ref.EPS * want.abs()).all()

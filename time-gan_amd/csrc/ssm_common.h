@@ -17,7 +17,10 @@ __device__ __forceinline__ float to_float(X v) { return (float)v; }
 template <typename X>
 __device__ __forceinline__ X from_float(float v) { return (X)v; }
 
-// 1 / (1 + exp(-v)) on the hardware exp2 / rcp units: about 2 ulp; 0 and 1 at the far ends.
+// 1 / (1 + exp(-v)) on the hardware exp2 / rcp units; 0 and 1 at the far ends.  The relative error below 0 is mostly that of
+// exp2's argument, a rounded product with a rounded constant: 1.22 |v| half steps, and about 5 from exp2, the sum and the
+// reciprocal; above 0 those 5 at most.  Measured, v sigmoid(v) against 64 bits: 2.8 half steps above 0, 5.7 at -5, 9.5 at -10,
+// 17 at -20, 64 at -80.
 __device__ __forceinline__ float sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
 }
