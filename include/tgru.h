@@ -471,7 +471,10 @@ size_t tgru_conv_backward_workspace_bytes(int B, int T, int D, int K);
  * state[slots[i]] (pool of P states (K-1, D) of `dtype`), whose rows move up by one and take x as the last; the new
  * state goes to state_out[slots[i]] (state_out == state: in place; any other overlap is an error of the caller).
  * slots: device int32[B], or NULL: row i has state i (then P >= B).  A row whose slot is outside [0, P) is padding:
- * y is 0 there and no state is touched.  Rows with the same slot are taken one after the other, in order of rows.
+ * y is 0 there and no state is touched.  Rows with the same slot are taken one after the other, in order of rows.  Every wave
+ * looks through all slots for that: the time of it grows with B squared (it shows from some thousand rows on), and calls whose
+ * search would take seconds (B B W >= 2^44; a row has W waves of 64 packs of 16 bytes, or of 64 channels where packs do not divide D;
+ * in tgru_scan_step of 256 states) are refused (TGRU_E_DIMS).
  */
 typedef struct tgru_conv_step_args {
     const void *x;

@@ -46,3 +46,17 @@ def test_convolutions_that_one_launch_holds_are_taken(tg):  # noqa: F811
         assert (lb.tgru_conv_backward_workspace_bytes(*dims, 4) > 0) == (want == E_NULL)
     for dtype, want in ((0, E_DIMS), (1, E_NULL), (2, E_NULL)):       # 2^32 and 2^31 packs of one step
         assert lb.tgru_conv_forward(ctypes.byref(ConvArgs(B=1 << 26, T=1, D=256, K=4, dtype=dtype)), None) == want
+
+
+def test_slots_that_would_be_searched_for_seconds_are_refused(tg):  # noqa: F811
+    """Rows squared times waves a row, below 2^44; without slots nothing is searched."""
+    import ctypes
+    from timegan_amd._lib import ConvStepArgs, ScanStepArgs
+    lb, E_DIMS, E_NULL = tg.lib(), -1, -2
+    conv = lambda B, D, slots=16, dtype=0: lb.tgru_conv_step(ctypes.byref(ConvStepArgs(B=B, P=B, D=D, K=4, slots=slots, dtype=dtype)), None)  # noqa: E731
+    assert conv(1 << 21, 256) == E_NULL and conv(1 << 22, 256) == E_DIMS and conv(1 << 22, 256, None) == E_NULL
+    assert conv(1 << 21, 257) == E_DIMS and conv(1 << 20, 257) == E_NULL                # five waves a row
+    assert conv(1 << 21, 512, dtype=1) == E_NULL and conv(1 << 21, 1024) == E_DIMS
+    scan = lambda B, D, slots=16: lb.tgru_scan_step(ctypes.byref(ScanStepArgs(B=B, P=B, D=D, N=16, G=1, slots=slots)), None)  # noqa: E731
+    assert scan(1 << 21, 16) == E_NULL and scan(1 << 22, 16) == E_DIMS and scan(1 << 22, 16, None) == E_NULL
+    assert scan(1 << 19, 1024) == E_DIMS and scan((1 << 19) - 1, 1024) == E_NULL

@@ -1152,7 +1152,7 @@ int tgru_scan_step(const tgru_scan_step_args *a, tgru_stream_t stream) {
     if (!a->slots && a->P < a->B) return TGRU_E_DIMS;
     // less than 2^32 threads
     const int CH = 256 / (a->N <= 4 ? 4 : padded_states(a->N)), tpg = (a->D / a->G - 1) / CH + 1;
-    if ((double)a->B * tpg * a->G >= 67108860.0) return TGRU_E_DIMS;
+    if ((double)a->B * tpg * a->G >= 67108860.0 || search_too_long(a->slots, a->B, (long)tpg * a->G)) return TGRU_E_DIMS;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     if (!a->u || !a->delta || !a->b || !a->c || !a->a || !a->state || !a->state_out || !a->y) return TGRU_E_NULL;
     if (int rc = tgru::check_device()) return rc;

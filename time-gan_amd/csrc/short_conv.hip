@@ -386,11 +386,17 @@ int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
     return hipGetLastError() == hipSuccess ? TGRU_OK : TGRU_E_LAUNCH;
 }
 
+// Waves a row of the one-token form: packs where they divide D (no shared channels: the state may be updated where it lies).
+int step_blocks(int D, int dtype) {
+    const int vec = 16 / (int)dtype_bytes(dtype);
+    return ((D % vec == 0 ? D / vec : D) + 63) / 64;
+}
+
 template <typename X, int K>
 int run_conv_step(const tgru_conv_step_args &a, hipStream_t s) {
     constexpr int VEC = 16 / (int)sizeof(X);
-    const bool packs = a.D % VEC == 0;       // (no shared channels here: the state may be updated where it lies)
-    const int nvec = packs ? a.D / VEC : a.D, nblk = (nvec + 63) / 64;
+    const bool packs = a.D % VEC == 0;
+    const int nvec = packs ? a.D / VEC : a.D, nblk = step_blocks(a.D, a.dtype);
     const dim3 grid((unsigned)((long)a.B * nblk)), block(64);
     if (packs) TGRU_LAUNCH((conv_step_kernel<X, K, VEC>), grid, block, 0, s, a, nvec, nblk);
     else TGRU_LAUNCH((conv_step_kernel<X, K, 1>), grid, block, 0, s, a, nvec, nblk);
@@ -480,6 +486,7 @@ int tgru_conv_step(const tgru_conv_step_args *a, tgru_stream_t stream) {
     // less than 2^32 threads
     if (a->D > (1 << 30) || (long)a->B * ((a->D + 63) / 64) >= (1L << 26) || (!a->slots && a->P < a->B)) return TGRU_E_DIMS;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
+    if (search_too_long(a->slots, a->B, step_blocks(a->D, a->dtype))) return TGRU_E_DIMS;
     if (!a->x || !a->weight || !a->y || (a->K > 1 && (!a->state || !a->state_out))) return TGRU_E_NULL;
     if (int rc = tgru::check_device()) return rc;
     return dispatch_conv_step(*a, (hipStream_t)stream);

@@ -46,7 +46,9 @@ __device__ __forceinline__ int clamped_length(const int32_t *lengths, int b, int
 }
 
 // The first row j in [from, to) with slots[j] == slot, or `to`.  All 64 lanes of the wave call it with the same
-// arguments; 256 rows are looked at per trip, their loads in flight together.
+// arguments; 256 rows are looked at per trip, their loads in flight together.  Every wave of every row goes through all slots,
+// so a call's search grows with the square of its rows.  Measured, scan with 256 channels (16 waves a row), fp32, 16 states:
+// nothing at 300 rows, 30 us become 98 at 4096, 0.4 ms become 15 at 65536, 0.8 become 59 at 131072.
 __device__ __forceinline__ int find_slot(const int32_t *__restrict__ slots, int from, int to, int slot) {
     const int lane = threadIdx.x & 63;
     for (int base = from; base < to; base += 256) {
@@ -83,6 +85,11 @@ __device__ __forceinline__ float sum_rows(const float *__restrict__ p, long stri
 #pragma unroll
         for (int q = 0; q < w; ++q) s[q] += s[q + w];
     return s[0];
+}
+
+// Whether a one-token call with slots is refused because its search would take seconds (2^44 row pairs and waves: about 4 s).
+inline bool search_too_long(const int32_t *slots, int B, long waves_per_row) {
+    return slots && (double)B * B * waves_per_row >= 17592186044416.0;
 }
 
 inline bool known_dtype(int dtype) { return dtype == TGRU_DTYPE_F32 || dtype == TGRU_DTYPE_BF16 || dtype == TGRU_DTYPE_F16; }

@@ -83,7 +83,8 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     state (P, K - 1, D) in x's type, dense, is a pool of states; row i of x belongs to state[slots[i]] (state[i] without
     slots).  The states are updated in place, or written to state_out (same shape) with `state` left as it was.  A row
     whose slot is outside [0, P) is padding: y is 0, no state is touched.  Rows with the same slot are steps of one sequence
-    and are taken in order.  slots: dense int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
+    and are taken in order; looking for them costs time that grows with the square of the rows (little up to some thousand
+    rows, 15 ms at 65536; what would take seconds is refused).  slots: dense int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
     not overlap the states that are written (refused).  No backward pass.
     """
     return _op().short_conv_step(x, state, weight, bias, silu, _slots(slots, x.device), state_out)
