@@ -493,7 +493,8 @@ int tgru_conv_step(const tgru_conv_step_args *a, tgru_stream_t stream);
  *     dt_t = softplus(delta_t + delta_bias)        (delta_t + delta_bias without `softplus`)
  *     h_t  = exp(dt_t A[d]) h_{t-1} + dt_t u_t b_t[group of d]
  *     y_t  = (c_t[group of d] . h_t + skip[d] u_t) z_t / (1 + exp(-z_t))
- * States may grow (dt A > 0): they and their gradients, and exp(dt_t A) of ONE step, have to be float32 numbers.
+ * States may grow (dt A > 0): they and their gradients, and exp(dt_t A) of ONE step, have to be float32 numbers.  A rate of
+ * -infinity forgets the state at every step of dt > 0.  Infinite values of a sequence's own steps may come out as NaN.
  * a (D, N); 1 <= N <= TGRU_SCAN_MAX_STATES; G divides D, group of d = d / (D / G).  skip, delta_bias and z may be NULL
  * (no such term / factor).  initial_state / final_state (B, D, N) fp32, NULL: zeros / not wanted.
  * reserve: tgru_scan_reserve_bytes() bytes that the backward call reads, or NULL (inference).

@@ -2,10 +2,9 @@
 // ONE SEQUENCE PER WORKGROUP, matrix-vector products on the vector ALU.
 //
 // Why not MFMA here: an MFMA tile needs 16 sequences per workgroup, so a batch of 128 occupies 8 of
-// the 256 CUs and every time step pays for a 16-column tile (about 2 us per step).  The fp32 packed
-// FMA rate of the vector ALU equals the fp32 MFMA rate on this chip, and with one sequence per
-// workgroup the same batch spreads over 128 CUs, each doing a 72x48 matrix-vector product per layer
-// and step (36 packed FMAs per lane).  The time step, which is what bounds a recurrence this small,
+// the 256 CUs and every time step pays for a 16-column tile (about 2 us per step).  With one sequence
+// per workgroup the same batch spreads over 128 CUs, each doing a 72x48 matrix-vector product per layer
+// and step (72 multiply-adds per lane).  The time step, which is what bounds a recurrence this small,
 // becomes several times shorter.  Above a few thousand sequences the MFMA kernels win again.
 //
 // Layout of one workgroup: one COMPUTE wave per layer (layers run as a wavefront: wave l works on

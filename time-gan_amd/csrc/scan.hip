@@ -6,8 +6,10 @@
 // eighteen operations and the exponential backward, against a few bytes per channel: with 16 states the vector ALU and
 // not HBM is the limit.  The matrix instructions do not apply: every (channel, state) pair has a decay of its own at
 // every step, so no product of two matrices is shared by two steps.  What the vector ALU of this chip does in how many
-// cycles per wave (measured, two or more waves per SIMD): 4-byte multiplies, adds and multiply-adds 2.5, 8-byte ones,
-// DPP adds, selects and conversions 4.3, exp2 / log2 / reciprocal 8.2, permlane swaps 8.3; with one wave, 5 at least.
+// cycles per wave (measured, two or more waves per SIMD): multiplies, adds and multiply-adds 2.3 (4 where both factors are one
+// register), DPP adds 4.3, exp2 / reciprocal 8.2, permlane swaps 8.3; with one wave, 4.6 at least.  Between exponentials the
+// short ones gain less: three and an exponential take 18.8, not 15.  The four states' arithmetic of a step, measured alone with
+// everything in registers, takes a SIMD 37 ns a wave forward (88 cycles), 35 in the pass for the chunks' ends and 155 backward.
 // So: enough waves, operands that fit the short encodings, few selects, and no instruction for what is the same in a
 // whole wave.
 //
@@ -16,7 +18,7 @@
 // what is per channel only (softplus, dt u, the gate) is computed once per (step, channel) by lanes that split the block
 // among themselves, the maps' rows are brought to fp32; the next block's rows are requested before the recurrence runs
 // over this one.  (Tried instead: a lane with all 16 states of a channel and the maps through the scalar cache -- an eighth
-// fewer instructions, but a quarter of the waves: 139 us against 91 on a batch of 64 windows of 256 steps with 1024
+// fewer instructions, but a quarter of the waves: half as slow again on a batch of 64 windows of 256 steps with 1024
 // channels, equal on one sequence of 16384.)
 //
 // scan_bwd_kernel needs the states of every step in reverse.  The forward pass saves the state in front of every block
@@ -284,10 +286,12 @@ struct Lane {
 __device__ __forceinline__ void unpack(const float4 &f, float (&v)[4]) { v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w; }
 
 // MODE 0: the outputs.  MODE 1: a chunk's end state from a zero start and its sum of dt, for the joining kernel.
-// Bound by the vector ALU's issue: 28 instructions a wave and step (21 in MODE 1), of which 20 (16) are the four states'
-// arithmetic; it is busy in 96 % of the cycles of the second case below, in 81 % of the first.  Measured, 16 states: 64 windows of 256 steps, 1024 channels, fp32, 91 us
-// (3.7 TB/s); one sequence of 16384 steps, 2048 channels, bf16, in 32 chunks: 147 us, MODE 1 105 us and the joining 6.
-// Taking the exponentials out of the latter (wrong results) leaves 112 + 67 us, the maps' LDS reads 147 + 106.
+// 28 instructions a wave and step (21 in MODE 1), of which 20 (17) are the four states' arithmetic.  Measured, 16 states: one
+// sequence of 16384 steps, 2048 channels, bf16, in 32 chunks: 140 us, MODE 1 100 us and the joining 6, which is 68 and 49 ns a
+// wave and step of a SIMD with four waves where that arithmetic alone takes 37 and 35.  The other instructions are some 15 and 8 ns
+// at their rates; the rest is waiting, though not for the maps: a copy that read one row of them for all steps was no faster,
+// one without any of a step's LDS reads by 3 %, one without the exponentials by 22 % (MODE 1 by 35 %).  64 windows of 256
+// steps, 1024 channels, fp32: 88 us, 86 ns a wave and step, 3.8 TB/s, so memory counts there as well.
 template <typename X, int S, int MODE>
 __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64, M = MODE == 0 ? 2 : 1;
@@ -419,7 +423,7 @@ __global__ __launch_bounds__(64 * kWaves) void scan_fwd_kernel(tgru_scan_args a,
 }
 
 // The gradient that a chunk hands to the one before it, from zero behind its end, and its sum of dt: MODE 1 above from the
-// other end, with c dy in the place of b dt u.  60 us for 4 sequences of 2048 steps, 2048 channels, bf16.
+// other end, with c dy in the place of b dt u.  54 us for 4 sequences of 2048 steps, 2048 channels, bf16.
 template <typename X, int S>
 __global__ __launch_bounds__(64 * kWaves) void scan_back_kernel(tgru_scan_args a, Plan pl, float *carry, float *sdt) {
     constexpr int CH = 64 / S, NP = 4 * S, E = Q * CH / 64;
@@ -543,13 +547,15 @@ __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const flo
 // where dy is the gradient in front of the gate.  The four waves of a workgroup are neighbouring waves of one group, one
 // sequence and one chunk: their sums over channels are joined in LDS and one row per workgroup goes to memory.
 //
-// Bound by the vector ALU's issue as well: 101 instructions a wave and step, busy in 83 % of the cycles, two waves a SIMD
-// (the states and decays of R steps are 64 registers; with bounds for three waves it spills and takes 420 us).  Measured:
-// 64 windows of 256 steps, 1024 channels, 16 states, fp32, 275 us; what is taken out of it (wrong results) saves: the sums
-// over channels 45 us, the exponentials 27, stores and their arithmetic 28, the first half's second run 20, the sums over
-// states and softplus 12 each, the joining of the four waves 7.  R = 4 is slower (289 us), and so are sums over channels
-// exchanged through LDS (318).  With N <= 8 (S = 2) a lane has twice the work per channel and the compiler spills 30 to 55
-// registers outside the loops over steps: such a call takes about as long as one with 16 states.
+// 101 instructions a wave and step, of which 83 are the four states' arithmetic and its sums, with two waves a SIMD (the
+// states and decays of R steps are 64 registers; with bounds for three waves it spills and is half as slow again).  Measured: 64
+// windows of 256 steps, 1024 channels, 16 states, fp32, 260 us; 4 sequences of 2048 steps, 2048 channels, bf16, 240 us: 254 and
+// 234 ns a wave and step where that arithmetic alone takes 155 with two waves.  Some 35 ns are the other instructions at their rates,
+// the rest is waiting that two waves do not cover (a step's sums are chains of seven instructions).  Of 275 us that an earlier
+// run took, copies without one part each (wrong results) saved: the sums over channels 45 us, the exponentials 27, stores and
+// their arithmetic 28, the first half's second run 20, the sums over states and softplus 12 each, the joining of the four waves 7;
+// R = 4 took 289, sums over channels exchanged through LDS 318.  With N <= 8 (S = 2) a lane has twice the work per channel and the
+// compiler spills 30 to 55 registers outside the loops over steps: such a call takes about as long as one with 16 states.
 template <typename X, int S>
 __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args a, Plan pl, const float *carry, float *map_part,
                                                               float *par_part) {
@@ -858,7 +864,7 @@ __global__ __launch_bounds__(256) void scan_grads_kernel(tgru_scan_args a, Plan 
 }
 
 // One token: a wave takes CH channels of one row.  Bound by the states, read and written once: four of them a lane, in one
-// load where N is a multiple of 4 (256 rows of 4096 channels with 16 states: 37 us, 3.8 TB/s; one row of 1024: 3.3 us, a
+// load where N is a multiple of 4 (256 rows of 4096 channels with 16 states: 38 us, 3.8 TB/s; one row of 1024: 3.2 us, a
 // chain of three loads).  Rows with one slot are taken in order by the first one's wave.  A wave lives for little
 // more than its chain of dependent loads, so everything whose address does not depend on the slot is requested behind the
 // slot's own load, and the states before the search for an earlier row with this slot.
@@ -967,7 +973,8 @@ double pass_time(long waves, long steps, const double *cost, int most) {
 
 // Chunks of time: the number that the times measured below give the shortest pass for.  A chunk more costs the main pass
 // nothing but blocks cut short; the pass in front does more of its work again (all chunks but one), and with the joining
-// costs two launches.  Measured (16 states, us a step): one sequence more or less than a round matters most -- 14 and 16
+// costs two launches.  Measured with 16 states and sequences of full length (us a step), and used for all: fewer states a channel
+// spill in the backward pass, and sequences of unequal length end before the time that is planned for.  One sequence more or less than a round matters most -- 14 and 16
 // sequences (1792 and 2048 waves) of the backward pass take the same 503 us for 1024 steps, 20 take 708.
 Plan make_plan(int B, int T, int D, int N, int G, bool backward) {
     Plan p;

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(kConvThreads) void conv_fwd_kernel(tgru_conv_args a
 // A run looks K - 1 steps past its end (dx there needs them; they count towards dw in the run that owns them).  The
 // sums over a run's steps stay in registers; every run leaves one row (K + 1, D) of them, which a second kernel adds
 // up in a fixed order.  Registers decide here (taps, two windows and the sums are 140 floats a lane): two rows at a time
-// and the next two on their way took 95 us where four rows without that took 107 and eight 150.
+// and the next two on their way took 95 us where, in the same run, four rows without that took 107 and eight 150.
 template <typename X, int K, int VEC>
 __global__ __launch_bounds__(kConvThreads) void conv_bwd_kernel(tgru_conv_args a, int nvec, int runs, int run_len) {
     const Place p = place_of<VEC>(a, nvec, runs, run_len);
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(1024) void conv_param_grad_kernel(const float *__re
     else if (dweight) dweight[(long)d * K + k] = v;
 }
 
-// One token: a wave takes 64 VEC channels of one row (256 rows of 4096 channels in 16 bits: 7 us; one row of 1024: 2.4 us,
+// One token: a wave takes 64 VEC channels of one row (256 rows of 4096 channels in 16 bits: 7 us; one row of 1024: 2.2 us,
 // a chain of two or three loads).  Of the rows with one slot the first takes them all, in order,
 // with the state in registers between them; the others' waves find that they are not the first and leave.
 template <typename X, int K, int VEC>
@@ -330,8 +330,8 @@ __global__ __launch_bounds__(64) void conv_step_kernel(tgru_conv_step_args a, in
 }
 
 // Steps per run: as long as the launch still has about `waves` waves, because the K - 1 rows around a run are read twice; 8 at
-// least (one group of loads), 64 at most.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 48 us with 2048
-// waves (5.5 TB/s), 58 with 4096, 71 with 8192; backward 95 us with 2048 (4.2 TB/s).
+// least (one group of loads), 64 at most.  Measured, 8 x 4096 steps of 2048 channels in 16 bits: forward 55 us with 2048
+// waves (4.9 TB/s), a fifth more with 4096, half as much again with 8192; backward 106 us with 2048 (3.8 TB/s).
 int conv_run_len(int B, int T, int nvec, long waves) {
     int len = 64;
     while (len > 8 && (long)B * ((T + len - 1) / len) * nvec < waves * 64) len >>= 1;
@@ -347,7 +347,7 @@ int conv_vec(int D, int dtype) {
 }
 
 // Whether the rows of partial sums are folded first: more than four round trips a thread otherwise, and columns for less than
-// half of the chip.  Measured, in one launch / folded: 2048 rows of 240 columns 6.2 / 7.7 us, 3072 rows of 960 columns 8.8 / 7.6.
+// half of the chip.  Measured, in one launch / folded: 2048 rows of 240 columns 6.2 / 7.7 us, half as many again of 960 columns 8.8 / 7.6.
 bool conv_folds(long rows, long cols) { return rows > 4 * kFold && cols < 128 * 32; }
 int conv_fold(long rows) { return (int)std::max<long>(kFold, (rows + kMaxFolds - 1) / kMaxFolds); }
 

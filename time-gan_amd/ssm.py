@@ -68,7 +68,7 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     (list, CPU tensor, or an integer GPU tensor, which is not looked at on the host); outputs behind a sequence's end are
     0, inputs there are ignored whatever they hold, and no gradient goes there.
     Returns y (B, T, D), or (y, state) with return_state: the last K - 1 inputs of each sequence, the next call's
-    initial_state and what short_conv_step goes on from.  Differentiable once in every floating argument.
+    initial_state and what short_conv_step goes on from.  Differentiable once (in backward mode) in every floating argument.
     """
     if x.dim() == 3:
         lengths = _lengths(lengths, x.shape[0], x.shape[1], x.device)
@@ -84,8 +84,8 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     slots).  The states are updated in place, or written to state_out (same shape) with `state` left as it was.  A row
     whose slot is outside [0, P) is padding: y is 0, no state is touched.  Rows with the same slot are steps of one sequence
     and are taken in order; looking for them costs time that grows with the square of the rows (little up to some thousand
-    rows, 15 ms at 65536; what would take seconds is refused).  slots: dense int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
-    not overlap the states that are written (refused).  No backward pass.
+    rows, 15 ms for a scan of 65536 rows; what would take seconds is refused).  slots: dense int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
+    not overlap the states that are written (refused).  No derivatives.
     """
     return _op().short_conv_step(x, state, weight, bias, silu, _slots(slots, x.device), state_out)
 
@@ -104,8 +104,9 @@ def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: tor
     channels share them (one group: unsqueeze(2)); D, delta_bias (channels).  D, z, delta_bias may be None.
     initial_state (batch, channels, N) float32 or zeros.  lengths and padding as in short_conv; a sequence of length 0
     keeps its initial state.
+    States may grow (negative steps, positive rates) as far as float32 holds them and exp(dt A) of one step.
     Returns y, or (y, state) with return_state: the float32 state behind each sequence's last step.  Differentiable once
-    in every floating argument.
+    (in backward mode) in every floating argument.
     """
     if u.dim() == 3:
         lengths = _lengths(lengths, u.shape[0], u.shape[1], u.device)
@@ -119,7 +120,7 @@ def selective_scan_step(u: torch.Tensor, delta: torch.Tensor, state: torch.Tenso
                         state_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One more step of selective_scan for each of B sequences: u, delta, z (B, channels), B, C (B, G, N) -> y (B, channels).
     state (P, channels, N) float32, dense: a pool of states; slots, state_out, padding and repeated slots as in
-    short_conv_step.  No backward pass."""
+    short_conv_step.  No derivatives."""
     return _op().selective_scan_step(u, delta, state, A, B, C, D, z, delta_bias, softplus, _slots(slots, u.device), state_out)
 
 
