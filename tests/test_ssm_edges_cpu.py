@@ -39,6 +39,7 @@ def test_convolutions_that_one_launch_holds_are_taken(tg):  # noqa: F811
     lb, E_DIMS, E_NULL = tg.lib(), -1, -2
     for dims, want in (((32, 131072, 8192), E_NULL), ((520, 4096, 8192), E_NULL), ((1 << 20, 4096, 64), E_NULL), ((1 << 27, 1, 64), E_NULL),
                        ((1, 8, (1 << 31) - 256), E_NULL), ((1, 8, (1 << 31) - 255), E_DIMS), ((1, 1, (1 << 31) - 1), E_DIMS),
+                       (((1 << 31) - 256, 1, 1), E_NULL), (((1 << 31) - 255, 1, 1), E_DIMS), (((1 << 31) - 1, 1, 1), E_DIMS),
                        ((1 << 30, 128, 1), E_DIMS), ((1 << 29, 64, 64), E_DIMS), ((1 << 28, 64, 256), E_DIMS)):
         for dtype in (0, 1, 2):
             args = ctypes.byref(ConvArgs(**dict(zip("BTD", dims)), K=4, dtype=dtype))

@@ -131,3 +131,19 @@ def test_accuracy_of_the_activation(tg):  # noqa: F811
     y = tg.short_conv(v.view(-1, 1, 1).to(DEV), torch.ones(1, 1, device=DEV)).cpu().view(-1).double()
     want = v.double() * torch.sigmoid(v.double())
     assert ((y - want).abs() <= (7 - 1.22 * v.double().clamp(max=0)) * ref.EPS * want.abs()).all()
+
+
+def test_gradients_of_as_many_sequences_as_are_counted(tg):  # noqa: F811
+    """2^31 - 256 sequences of one step and one channel, all ones: rows of partial sums are numbered up to the end of 31 bits.  The
+    sums go through two rounds of at most 2^19 / 32 / 16 rows in a partial sum (whole numbers below 2^24, exact), 16 partial sums
+    and 32 threads, then 4096 rows: less than 384 roundings."""
+    B = 2 ** 31 - 256
+    one = torch.ones(1, 1, 1, device=DEV).expand(B, 1, 1)
+    w, b = torch.full((1, 1), 2.0, device=DEV, requires_grad=True), torch.ones(1, device=DEV, requires_grad=True)
+    y = tg.short_conv(one, w, b, silu=False)
+    assert bool((y == 3).all())
+    dw, db = torch.autograd.grad(y, (w, b), one)
+    for g in (dw, db):
+        assert abs(float(g) - B) <= 384 * ref.EPS * B
+    del y
+    torch.cuda.empty_cache()

@@ -372,7 +372,7 @@ int run_conv(const tgru_conv_args &a, bool backward, hipStream_t s) {
         const float *part = a.workspace;
         int rows = a.B * runs;
         if (conv_folds(rows, cols)) {
-            const int fold = conv_fold(rows), folds = (rows + fold - 1) / fold;
+            const int fold = conv_fold(rows), folds = (int)(((long)rows + fold - 1) / fold);
             float *folded = a.workspace + rows * cols;
             TGRU_LAUNCH(conv_param_grad_kernel<true>, dim3(blocks, (unsigned)folds), dim3(1024), 0, s, part, rows, a.D, K, nullptr, nullptr, folded,
                         fold);
@@ -427,13 +427,14 @@ int dispatch_conv_step(const tgru_conv_step_args &a, hipStream_t s) {
 #undef TGRU_CALL
 }
 
-// A launch has a thread for every run and pack, numbered in 32 bits, and the runs (rows of partial sums) are counted in 31.
+// A launch has a thread for every run and pack, numbered in 32 bits, and the runs (rows of partial sums) are counted in 31, with
+// room for a step beyond the last.
 int conv_dims(int B, int T, int D, int K, int dtype) {
     if (B <= 0 || T <= 0 || D <= 0 || K <= 0 || K > TGRU_CONV_MAX_TAPS) return TGRU_E_DIMS;
     if (T > (1 << 30) || D > INT32_MAX - kConvThreads + 1) return TGRU_E_DIMS;
     const int vec = conv_vec(D, dtype), nvec = (D + vec - 1) / vec, len = conv_run_len(B, T, nvec, kConvWaves);
     const double runs = (double)B * ((T + len - 1) / len);
-    return runs < 2147483648.0 && runs * nvec < 4294967296.0 - kConvThreads ? TGRU_OK : TGRU_E_DIMS;
+    return runs <= 2147483648.0 - kConvThreads && runs * nvec < 4294967296.0 - kConvThreads ? TGRU_OK : TGRU_E_DIMS;
 }
 
 }  // namespace ssm
