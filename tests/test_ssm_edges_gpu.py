@@ -147,3 +147,20 @@ def test_gradients_of_as_many_sequences_as_are_counted(tg):  # noqa: F811
         assert abs(float(g) - B) <= 384 * ref.EPS * B
     del y
     torch.cuda.empty_cache()
+
+
+def test_thousands_of_rows_with_slots_that_come_twice(tg):  # noqa: F811
+    """Rows i and 2500 + j with the same slot are two steps of one sequence: the same bits as two calls without repeats."""
+    g = torch.Generator().manual_seed(3)
+    P, D, N = 2500, 12, 8
+    first, second = torch.randperm(P, generator=g).to(DEV).int(), torch.randperm(P, generator=g).to(DEV).int()
+    x, u, delta, B, C = (randn(g, 2 * P, *s).to(DEV) for s in ((D,), (D,), (D,), (1, N), (1, N)))
+    w, A, cpool, pool = (randn(g, *s).to(DEV) for s in ((D, 4), (D, N), (P, 3, D), (P, D, N)))
+    A = -A.abs()
+    twice = [cpool.clone(), pool.clone()]
+    slots = torch.cat([first, second])
+    y = tg.short_conv_step(x, twice[0], w, slots=slots), tg.selective_scan_step(u, delta, twice[1], A, B, C, slots=slots)
+    for part, s in ((slice(0, P), first), (slice(P, 2 * P), second)):
+        assert torch.equal(tg.short_conv_step(x[part], cpool, w, slots=s), y[0][part])
+        assert torch.equal(tg.selective_scan_step(u[part], delta[part], pool, A, B[part], C[part], slots=s), y[1][part])
+    assert torch.equal(cpool, twice[0]) and torch.equal(pool, twice[1])

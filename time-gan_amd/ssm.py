@@ -84,8 +84,9 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     slots).  The states are updated in place, or written to state_out (same shape) with `state` left as it was.  A row
     whose slot is outside [0, P) is padding: y is 0, no state is touched.  Rows with the same slot are steps of one sequence
     and are taken in order; looking for them costs time that grows with the square of the rows (little up to some thousand
-    rows, 15 ms for a scan of 65536 rows; what would take seconds is refused).  slots: dense int32 GPU tensor (no copy), or whole numbers in anything torch.as_tensor takes.  x must
-    not overlap the states that are written (refused).  No derivatives.
+    rows, 15 ms for a scan of 65536 rows; what would take seconds is refused).  slots: dense int32 GPU tensor (no copy), or
+    whole numbers in anything torch.as_tensor takes.  x must not overlap the states that are written (refused).  No
+    derivatives.
     """
     return _op().short_conv_step(x, state, weight, bias, silu, _slots(slots, x.device), state_out)
 
