@@ -164,3 +164,19 @@ def test_thousands_of_rows_with_slots_that_come_twice(tg):  # noqa: F811
         assert torch.equal(tg.short_conv_step(x[part], cpool, w, slots=s), y[0][part])
         assert torch.equal(tg.selective_scan_step(u[part], delta[part], pool, A, B[part], C[part], slots=s), y[1][part])
     assert torch.equal(cpool, twice[0]) and torch.equal(pool, twice[1])
+
+
+def test_a_token_of_as_many_channels_as_are_counted(tg):  # noqa: F811
+    """2^31 - 1 channels of one state: the number of waves must not be rounded up beyond 31 bits."""
+    D = 2 ** 31 - 1
+    dev = torch.Generator(device=DEV).manual_seed(5)
+    u = torch.empty(1, D, dtype=torch.bfloat16, device=DEV).normal_(generator=dev)
+    A, state = torch.full((D, 1), -1.0, device=DEV), torch.ones(1, D, 1, device=DEV)
+    b = torch.ones(1, 1, 1, dtype=torch.bfloat16, device=DEV)
+    y = tg.selective_scan_step(u, u, state, A, b, b)
+    for part in (slice(0, 1000), slice(D // 2, D // 2 + 1000), slice(D - 1000, D)):
+        few = torch.ones(1, 1000, 1, device=DEV)
+        assert torch.equal(tg.selective_scan_step(u[:, part], u[:, part], few, A[:1000], b, b), y[:, part])
+        assert torch.equal(few, state[:, part])
+    del u, A, state, y
+    torch.cuda.empty_cache()

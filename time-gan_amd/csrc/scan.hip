@@ -1106,9 +1106,12 @@ int scan_call(const tgru_scan_args *a, bool backward, hipStream_t s) {
     return run_scan_states<_Float16>(*a, backward, s);
 }
 
+// Waves a group of the one-token form, of CH channels each.
+int step_tiles(int D, int G, int CH) { return (D / G - 1) / CH + 1; }
+
 template <typename X, int S>
 int run_scan_step(const tgru_scan_step_args &a, hipStream_t s) {
-    const int CH = 64 / S, tpg = (a.D / a.G + CH - 1) / CH, tiles = tpg * a.G;
+    const int tpg = step_tiles(a.D, a.G, 64 / S), tiles = tpg * a.G;
     auto ok = [](const void *p, size_t align) { return (uintptr_t)p % align == 0; };
     const bool quads = a.N % 4 == 0 && ok(a.state, 16) && ok(a.state_out, 16) && ok(a.a, 16) && ok(a.b, 4 * sizeof(X)) &&
                       ok(a.c, 4 * sizeof(X)) && a.b_stride[0] % 4 == 0 && a.b_stride[1] % 4 == 0 && a.c_stride[0] % 4 == 0 &&
@@ -1158,7 +1161,7 @@ int tgru_scan_step(const tgru_scan_step_args *a, tgru_stream_t stream) {
     if (a->B <= 0 || a->P <= 0 || a->D <= 0 || a->N <= 0 || a->G <= 0 || a->N > TGRU_SCAN_MAX_STATES || a->D % a->G) return TGRU_E_DIMS;
     if (!a->slots && a->P < a->B) return TGRU_E_DIMS;
     // less than 2^32 threads
-    const int CH = 256 / (a->N <= 4 ? 4 : padded_states(a->N)), tpg = (a->D / a->G - 1) / CH + 1;
+    const int tpg = step_tiles(a->D, a->G, 256 / (a->N <= 4 ? 4 : padded_states(a->N)));
     if ((double)a->B * tpg * a->G >= 67108860.0 || search_too_long(a->slots, a->B, (long)tpg * a->G)) return TGRU_E_DIMS;
     if (!known_dtype(a->dtype)) return TGRU_E_DTYPE;
     if (!a->u || !a->delta || !a->b || !a->c || !a->a || !a->state || !a->state_out || !a->y) return TGRU_E_NULL;
