@@ -180,3 +180,14 @@ def test_a_token_of_as_many_channels_as_are_counted(tg):  # noqa: F811
         assert torch.equal(few, state[:, part])
     del u, A, state, y
     torch.cuda.empty_cache()
+
+
+def test_sequences_refuse_dual_tensors(tg):  # noqa: F811
+    import torch.autograd.forward_ad as fw
+    x, w = torch.zeros(2, 3, 8, device=DEV), torch.zeros(8, 4, device=DEV)
+    b = torch.zeros(2, 3, 1, 4, device=DEV)
+    with fw.dual_level(), torch.no_grad():
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for call in (lambda: tg.short_conv(dual, w), lambda: tg.selective_scan(dual, x, w, b, b)):
+            with pytest.raises(RuntimeError, match="jvp is not implemented"):
+                call()
