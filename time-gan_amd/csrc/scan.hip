@@ -555,7 +555,7 @@ __global__ __launch_bounds__(64) void scan_join_kernel(const float *a, const flo
 // run took, copies without one part each (wrong results) saved: the sums over channels 45 us, the exponentials 27, stores and
 // their arithmetic 28, the first half's second run 20, the sums over states and softplus 12 each, the joining of the four waves 7;
 // R = 4 took 289, sums over channels exchanged through LDS 318.  With N <= 8 (S = 2) a lane has twice the work per channel and the
-// compiler spills 30 to 55 registers outside the loops over steps: such a call takes about as long as one with 16 states.
+// compiler spills 31 to 39 registers outside the loops over steps: such a call takes about as long as one with 16 states.
 template <typename X, int S>
 __global__ __launch_bounds__(64 * kWaves, 2) void scan_bwd_kernel(tgru_scan_args a, Plan pl, const float *carry, float *map_part,
                                                               float *par_part) {
